@@ -4,9 +4,7 @@
 // models/memory_bank.py:58-72 (truncating ring push), track_ssl/moco.py:152-156 (queue logits).
 #include <hip/hip_runtime.h>
 #include <math.h>
-#include <stdarg.h>
 #include <stdint.h>
-#include <stdio.h>
 #include <string.h>
 
 #include <atomic>
@@ -14,6 +12,7 @@
 #include <vector>
 
 #include "../../include/mi_knn.h"
+#include "host_common.h"
 #include "moco_kernel.h"
 #include "select_kernel.h"
 #include "sim_kernel.h"
@@ -21,25 +20,6 @@
 #include "vote_kernel.h"
 
 namespace {
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char *fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-#define HIP_CHECK(expr)                                                                   \
-    do {                                                                                  \
-        hipError_t e_ = (expr);                                                           \
-        if (e_ != hipSuccess)                                                             \
-            return fail(MI_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), \
-                        __FILE__, __LINE__);                                              \
-    } while (0)
 
 // ---- optional per-launch timing (bench.py's roofline leg).  Off by default; when on, every
 // similarity-kernel launch is bracketed by HIP events on ITS OWN stream.  Debug facility: guarded
@@ -70,24 +50,6 @@ struct ProfScope {
         g_prof.push_back(r);
     }
 };
-
-inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// A kernel that needs more dynamic LDS than the default limit has that limit raised ONCE per device (bit d of `done`:
-// device ordinal d), not on every call: hipFuncSetAttribute is a driver call on the launch path otherwise.
-template <typename Kernel>
-hipError_t ensure_dynamic_lds(Kernel kernel, size_t bytes, std::atomic<uint64_t> &done)
-{
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
-    if (bit && (done.load(std::memory_order_acquire) & bit)) return hipSuccess;
-    e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == hipSuccess && bit) done.fetch_or(bit, std::memory_order_release);
-    return e;
-}
 
 // --------------------------------------------------------------------------- small kernels
 // pack: float32 source -> compute dtype, K-contiguous rows, zero padded to ld_dst.
