@@ -10,15 +10,23 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MI_KNN_LIB") or os.path.join(HERE, "libmi_knn.so")   # override: experiments only
 
-MI_F32, MI_BF16 = 0, 1
+MI_F32, MI_BF16, MI_F16 = 0, 1, 2
 MI_MAX_K, MI_MAX_CLASSES = 1024, 65536
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 EXPORTS = [
     "mi_abi_version", "mi_last_error", "mi_profile_enable", "mi_profile_collect", "mi_profile_clock", "mi_debug_force_fallback", "mi_knn_ld", "mi_pack_rows", "mi_knn_topk_workspace_bytes", "mi_knn_topk_workspace_bytes_for_budget",
     "mi_knn_topk", "mi_knn_topk_static", "mi_knn_merge", "mi_knn_vote", "mi_queue_push", "mi_bank_scatter", "mi_moco_workspace_bytes",
     "mi_moco_fwd", "mi_moco_bwd", "mi_queue_push_stash", "mi_bank_append_normalized", "mi_queue_push_wrap", "mi_soft_knn_workspace_bytes", "mi_soft_knn", "mi_kth_largest",
+    "mi_cache_width", "mi_cache_push", "mi_cache_trim", "mi_cache_read", "mi_cache_attend_workspace_bytes", "mi_cache_attend",
+    "mi_cache_evict_workspace_bytes", "mi_cache_evict",
 ]
+
+
+class Cache(ctypes.Structure):
+    """``mi_cache_t``: the device pointers and sizes of one 4-bit cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("key", "key_scale", "value", "value_scale", "weight", "position", "length", "seen")] + \
+               [(n, ctypes.c_int64) for n in ("batch", "heads", "dim", "rows", "limit")]
 
 
 class MiKnnError(RuntimeError):
@@ -82,6 +90,20 @@ def lib() -> ctypes.CDLL:
     L.mi_moco_bwd.argtypes = [p, p, p, i64, i64, i64, f32, p, p, p, p, p, p, i64, i64, p, sz, p]
     L.mi_queue_push_stash.restype = i32
     L.mi_queue_push_stash.argtypes = [p, i64, i64, i64, p, i64, p, ctypes.POINTER(i64), p]
+    cache, strides = ctypes.POINTER(Cache), ctypes.POINTER(i64)
+    L.mi_cache_width.restype, L.mi_cache_width.argtypes = i64, [i64]
+    L.mi_cache_push.restype = i32
+    L.mi_cache_push.argtypes = [cache, p, strides, p, strides, i32, i64, p, p, p, p]
+    L.mi_cache_trim.restype, L.mi_cache_trim.argtypes = i32, [cache, p, i64, p]
+    L.mi_cache_read.restype, L.mi_cache_read.argtypes = i32, [cache, p, p, p]
+    L.mi_cache_attend_workspace_bytes.restype = sz
+    L.mi_cache_attend_workspace_bytes.argtypes = [cache, i32, i64, i64, i64, i32]
+    L.mi_cache_attend.restype = i32
+    L.mi_cache_attend.argtypes = [cache, p, strides, p, strides, i32, i64, i64, p, f32, i32, i32, i64, p, sz, p]
+    L.mi_cache_evict_workspace_bytes.restype = sz
+    L.mi_cache_evict_workspace_bytes.argtypes = [cache, i64]
+    L.mi_cache_evict.restype = i32
+    L.mi_cache_evict.argtypes = [cache, cache, i64, i64, p, sz, p]
     if L.mi_abi_version() != ABI_VERSION:
         raise MiKnnError(f"libmi_knn.so ABI {L.mi_abi_version()} != expected {ABI_VERSION}: rebuild")
     _lib = L

@@ -1,0 +1,290 @@
+"""A bank of key / value rows held in 4 bits on MI355X, read by softmax attention, that drops the rows that attention uses least.
+
+It stands next to ``MemoryBank`` (``models/memory_bank.py:35-72``: rows in whole floats, the oldest leave first, read by a dense product and
+a softmax as in ``track_semi/comatch.py:187-189``) and has no reference counterpart: rows belong to ``heads`` heads of ``batch`` sequences, as
+the keys and values of an attention layer do; ``heads=1, batch=1`` is a plain feature bank.
+
+    bank = CacheBank()
+    bank.register("layer0", dim=128, k=4096, heads=8, batch=64)
+    bank = bank.cuda()
+    bank.push("layer0", key, value)                            # [batch, heads, T, dim], quantised to 4.25 bits a value
+    out = bank.attend("layer0", query, accumulate=True)        # [batch, heads * group, T, dim]; also sums what each row got
+    bank.evict("layer0", keep=2048, recent=256)                # the least attended rows leave
+
+Storage is registered buffers (``<name>_key``, ``_key_scale``, ``_value``, ``_value_scale``, ``_weight``, ``_position``, ``_length``, ``_seen``;
+layouts and the number format in ``include/mi_knn.h``), so ``.to(device)`` and ``state_dict`` behave as for the other banks.  Each rank holds
+its own sequences: nothing is gathered.  No gradients: the bank is memory, as the MoCo queue is.  No CPU path.
+
+Lengths live on the device and no call waits for it, except a ``push`` that may run over: the host knows an upper bound of the lengths and
+reads them back when that bound plus the new rows passes ``k``.  All calls can be captured into a graph; a captured ``push`` cannot look,
+and rows that do not fit when it is replayed are dropped."""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch import nn
+
+from . import _lib
+
+__all__ = ["CacheBank"]
+
+_CODES = {torch.float32: _lib.MI_F32, torch.bfloat16: _lib.MI_BF16, torch.float16: _lib.MI_F16}
+_PARTS = ("key", "key_scale", "value", "value_scale", "weight", "position", "length", "seen")
+_DTYPES = (torch.uint8, torch.uint8, torch.uint8, torch.uint8, torch.float32, torch.int32, torch.int32, torch.int32)
+
+
+def _on(device: torch.device):
+    """The device's context, where it is not the current one already."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _strides(t: torch.Tensor):
+    """Strides of the sequence, head and row of a [batch, heads, rows, dim] tensor; a size of one has none."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where its rows are contiguous and start on 16 bytes, else a copy that is so."""
+    step = 16 // t.element_size()
+    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and not any(s % step for s in _strides(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class CacheBank(nn.Module):
+    """Named 4-bit banks of keys and values: ``register``, ``push``, ``attend``, ``evict``, ``trim``, ``bank[name]``."""
+
+    def __init__(self):
+        super().__init__()
+        self.sizes = {}            # name -> k
+        self.shapes = {}           # name -> (batch, heads, dim)
+        self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows
+        self._captured = set()     # names whose lengths a graph may change behind the host's back
+        self._views = {}           # name -> (buffers, mi_cache_t over them)
+
+    def __getstate__(self):
+        return {**self.__dict__, "_views": {}}
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._bounds = dict(self.sizes)
+
+    def register(self, name, dim, k, heads=1, batch=1, device=None):
+        """An empty bank of ``k`` rows of ``dim`` values (a multiple of 8, at most 256) for each head of each sequence."""
+        dim, k, heads, batch = int(dim), int(k), int(heads), int(batch)
+        if dim < 8 or dim > 256 or dim % 8:
+            raise ValueError(f"dim must be a multiple of 8 in [8, 256], got {dim}")
+        if k < 1 or heads < 1 or batch < 1:
+            raise ValueError(f"k, heads and batch must be positive, got k={k} heads={heads} batch={batch}")
+        width = 64 if dim <= 64 else 128 if dim <= 128 else 256
+        rows = (k + 63) // 64 * 64
+        held, scales = (batch, heads, rows, width // 2), (batch, heads, width // 32, rows)
+        for part, dtype, shape in zip(_PARTS, _DTYPES, (held, scales, held, scales, (batch, heads, rows), (batch, heads, rows), (batch,), (batch,))):
+            self.register_buffer(f"{name}_{part}", torch.zeros(shape, dtype=dtype, device=device))
+        self.sizes[name], self.shapes[name], self._bounds[name] = k, (batch, heads, dim), 0
+        self._captured.discard(name)
+        self._views.pop(name, None)
+
+    # ------------------------------------------------------------------------------------------------------------ helpers
+    def _cache(self, name, what):
+        if name not in self.sizes:
+            raise KeyError(f"CacheBank.{what}: no bank named {name!r}")
+        held = tuple(self._buffers[f"{name}_{part}"] for part in _PARTS)
+        known = self._views.get(name)
+        if known is not None and all(a is b for a, b in zip(known[0], held)):
+            return known[1], held
+        if not held[0].is_cuda:
+            raise RuntimeError(f"CacheBank.{what}: buffer is on {held[0].device}; image-classification_amd moves bank rows "
+                               "with HIP kernels only (no CPU fallback) -- call .to(device) first")
+        for part, dtype, t in zip(_PARTS, _DTYPES, held):
+            if t.dtype != dtype or not t.is_contiguous() or t.device != held[0].device:
+                raise RuntimeError(f"CacheBank.{what}: buffer {name}_{part} must be contiguous {dtype} on {held[0].device}, "
+                                   f"got {t.dtype} on {t.device} (move banks with .to(device), not to another dtype)")
+        batch, heads, dim = self.shapes[name]
+        view = _lib.Cache(*[t.data_ptr() for t in held], batch, heads, dim, held[4].shape[2], self.sizes[name])
+        self._views[name] = (held, view)
+        return view, held
+
+    @staticmethod
+    def _counts(counts, batch, T, device):
+        if counts is None:
+            return None
+        if not isinstance(counts, torch.Tensor):
+            values = [int(n) for n in counts]
+            if len(values) != batch or any(n < 0 or n > T for n in values):
+                raise ValueError(f"counts must be {batch} numbers in [0, {T}], got {values}")
+            return torch.tensor(values, dtype=torch.int32, device=device)
+        if counts.dtype not in (torch.int32, torch.int64) or tuple(counts.shape) != (batch,) or counts.device != device:
+            raise ValueError(f"counts must be {batch} int32 or int64 on {device}, got {counts.dtype} {tuple(counts.shape)} on {counts.device}")
+        return (counts if counts.dtype == torch.int32 else counts.clamp(0, T).to(torch.int32)).contiguous()
+
+    def _rows(self, what, name, t, arg, heads, device):
+        batch, _, dim = self.shapes[name]
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(f"{arg} must be a tensor on an MI355X (HIP) device: image-classification_amd has no CPU fallback")
+        if t.device != device:
+            raise RuntimeError(f"CacheBank.{what}: {arg} is on {t.device}, the bank on {device}")
+        if t.dtype not in _CODES:
+            raise ValueError(f"CacheBank.{what}: {arg} must be float32, bfloat16 or float16, got {t.dtype}")
+        if t.dim() != 4 or t.shape[0] != batch or t.shape[3] != dim or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"CacheBank.{what}: {arg} {tuple(t.shape)} does not fit a bank of {batch} sequences, {self.shapes[name][1]} heads, dim {dim} "
+                             "(expected [batch, heads, rows, dim])")
+        return t
+
+    def _changes(self, name) -> bool:
+        """Whether the call is being captured: from then on the host knows nothing about this bank's lengths."""
+        if torch.cuda.is_current_stream_capturing():
+            self._captured.add(name)
+            return True
+        return False
+
+    def _set_bound(self, name, bound):
+        self._bounds[name] = self.sizes[name] if name in self._captured else min(bound, self.sizes[name])
+
+    # --------------------------------------------------------------------------------------------------------------- calls
+    @torch.no_grad()
+    def push(self, name, key, value, counts=None, held=False):
+        """Appends ``key`` and ``value`` [batch, heads, T, dim] behind the last row of every sequence, quantised to 4 bits.
+
+        ``counts`` (one whole number for each sequence, a list or a tensor on the device): only the first ``counts[b]`` of the T rows
+        of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now holds for the two, in
+        their type and [batch, heads, T, dim], zeros where nothing was stored.  Raises ``RuntimeError`` before anything is written if a
+        sequence would pass ``k`` rows."""
+        view, held_by = self._cache(name, "push")
+        device = held_by[0].device
+        heads = self.shapes[name][1]
+        key = self._rows("push", name, key, "key", heads, device).detach()
+        value = self._rows("push", name, value, "value", heads, device).detach()
+        if key.shape != value.shape or key.dtype != value.dtype:
+            raise ValueError(f"CacheBank.push: key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} differ")
+        T, k = key.shape[2], self.sizes[name]
+        counts = self._counts(counts, key.shape[0], T, device)
+        with _on(device):
+            if not self._changes(name):
+                bound = k if name in self._captured else self._bounds[name]
+                if bound + T > k:                       # the one place that waits for the device
+                    lengths = held_by[6]
+                    longest = int((lengths if counts is None else lengths + counts.clamp(0, T)).max()) + (T if counts is None else 0)
+                    if longest > k:
+                        raise RuntimeError(f"CacheBank.push: {longest} rows do not fit bank {name!r} of {k}; evict or trim first")
+                    bound = longest - T if counts is None else longest
+                self._set_bound(name, bound + T)
+            else:
+                self._set_bound(name, k)
+            key, value = _aligned(key), _aligned(value)
+            out = tuple(torch.empty(key.shape, dtype=key.dtype, device=device) for _ in range(2)) if held else (None, None)
+            _lib.check(_lib.lib().mi_cache_push(ctypes.byref(view), key.data_ptr(), (ctypes.c_int64 * 3)(*_strides(key)),
+                                                value.data_ptr(), (ctypes.c_int64 * 3)(*_strides(value)), _CODES[key.dtype], T,
+                                                None if counts is None else counts.data_ptr(), None if not held else out[0].data_ptr(),
+                                                None if not held else out[1].data_ptr(), _lib.stream_ptr(device)), "mi_cache_push")
+        return out if held else None
+
+    def attend(self, name, query, counts=None, scale=None, causal=True, accumulate=False):
+        """Softmax attention of ``query`` [batch, heads * group, T, dim] over the bank, in the query's type and layout: query head h
+        reads head ``h // group``.
+
+        ``causal``: the query rows are the last rows of their sequence (push first, then attend), and row t does not see the rows after
+        its own; otherwise every row sees the whole sequence.  ``counts``: as in :meth:`push`, real rows of each sequence.  Rows that are not
+        real or see nothing give zeros.  ``scale``: positive, ``dim ** -0.5`` if not given.  ``accumulate`` adds to :meth:`weights` what
+        each row of the bank got, summed over query rows and the group's heads; :meth:`evict` goes by that."""
+        view, held_by = self._cache(name, "attend")
+        device = held_by[0].device
+        batch, heads, dim = self.shapes[name]
+        query = self._rows("attend", name, query, "query", None, device)
+        if query.shape[1] == 0 or query.shape[1] % heads:
+            raise ValueError(f"CacheBank.attend: {query.shape[1]} query heads are no multiple of the bank's {heads}")
+        if torch.is_grad_enabled() and query.requires_grad:
+            raise RuntimeError("CacheBank.attend has no gradient: call it under torch.no_grad() or with query.detach()")
+        scale = dim ** -0.5 if scale is None else float(scale)
+        query = query.detach()
+        T, group = query.shape[2], query.shape[1] // heads
+        counts = self._counts(counts, batch, T, device)
+        L = _lib.lib()
+        with _on(device):
+            query = _aligned(query)
+            out = torch.empty_like(query)
+            if out.stride(3) != 1 or any(s * out.element_size() % 16 for s in _strides(out)):
+                out = torch.empty(query.shape, dtype=query.dtype, device=device)
+            if T == 0:
+                return out
+            span = max(1, self.sizes[name] if name in self._captured else self._bounds[name])
+            code = _CODES[query.dtype]
+            nbytes = L.mi_cache_attend_workspace_bytes(ctypes.byref(view), code, T, group, span, int(accumulate))
+            ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+            _lib.check(L.mi_cache_attend(ctypes.byref(view), query.data_ptr(), (ctypes.c_int64 * 3)(*_strides(query)),
+                                         out.data_ptr(), (ctypes.c_int64 * 3)(*_strides(out)), code, T, group,
+                                         None if counts is None else counts.data_ptr(), scale, int(causal), int(accumulate), span,
+                                         ws.data_ptr(), ws.numel(), _lib.stream_ptr(device)), "mi_cache_attend")
+        return out
+
+    @torch.no_grad()
+    def evict(self, name, keep, recent=0, into=None):
+        """Cuts every head of every sequence down to ``keep`` rows: those among the last ``recent`` pushed of the sequence stay, then those
+        with the largest :meth:`weights`, ties to the lower slot.  Slots below ``keep`` whose row leaves take, in ascending order, the kept
+        rows from above.  ``into``: the rows that stay go to that bank (same batch, heads, dim, at least ``keep`` rows; what it held is
+        gone) and this one is left as it was."""
+        view, held_by = self._cache(name, "evict")
+        device = held_by[0].device
+        target, keep, recent = name if into is None else into, int(keep), int(recent)
+        if into == name:
+            raise ValueError("CacheBank.evict: into must name another bank (leave it out to evict in place)")
+        other = view if into is None else self._cache(into, "evict")[0]
+        if into is not None and (self.shapes[into] != self.shapes[name] or self._buffers[f"{into}_key"].device != device):
+            raise ValueError(f"CacheBank.evict: bank {into!r} {self.shapes[into]} does not match bank {name!r} {self.shapes[name]} (batch, heads, dim) on {device}")
+        if keep < 1 or keep > self.sizes[target]:
+            raise ValueError(f"CacheBank.evict: keep={keep} outside [1, {self.sizes[target]}]")
+        if recent < 0 or recent > keep:
+            raise ValueError(f"CacheBank.evict: recent={recent} outside [0, keep={keep}]")
+        L = _lib.lib()
+        with _on(device):
+            self._changes(target)
+            ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(ctypes.byref(view), keep)), dtype=torch.uint8, device=device)
+            _lib.check(L.mi_cache_evict(ctypes.byref(view), ctypes.byref(other), keep, recent, ws.data_ptr(), ws.numel(),
+                                        _lib.stream_ptr(device)), "mi_cache_evict")
+        self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bounds[name]))
+
+    @torch.no_grad()
+    def trim(self, name, lengths=0):
+        """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
+        the bank, a smaller length takes back the rows pushed last (a rejected draft).  Positions go on from the cut."""
+        view, held_by = self._cache(name, "trim")
+        device = held_by[0].device
+        each, number = None, 0
+        if isinstance(lengths, torch.Tensor):
+            top = torch.iinfo(torch.int32).max
+            each = self._counts(lengths, self.shapes[name][0], top, device)
+        else:
+            number = int(lengths)
+            if number < 0:
+                raise ValueError(f"CacheBank.trim: lengths must not be negative, got {number}")
+            number = min(number, self.sizes[name])
+        with _on(device):
+            self._changes(name)
+            _lib.check(_lib.lib().mi_cache_trim(ctypes.byref(view), None if each is None else each.data_ptr(), number,
+                                                _lib.stream_ptr(device)), "mi_cache_trim")
+        self._set_bound(name, self._bounds[name] if each is not None else min(number, self._bounds[name]))
+
+    @torch.no_grad()
+    def __getitem__(self, name):
+        """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""
+        view, held_by = self._cache(name, "__getitem__")
+        device = held_by[0].device
+        batch, heads, dim = self.shapes[name]
+        with _on(device):
+            out = tuple(torch.empty((batch, heads, self.sizes[name], dim), dtype=torch.bfloat16, device=device) for _ in range(2))
+            _lib.check(_lib.lib().mi_cache_read(ctypes.byref(view), out[0].data_ptr(), out[1].data_ptr(), _lib.stream_ptr(device)), "mi_cache_read")
+        return out
+
+    def lengths(self, name):
+        """Rows in use of each sequence: the bank's own int32 [batch] buffer (to read, not to write)."""
+        return self._buffers[f"{name}_length"]
+
+    def weights(self, name):
+        """Attention that each row got since it was pushed, float32 [batch, heads, k]; slots from the length on hold nothing of meaning."""
+        return self._buffers[f"{name}_weight"][..., :self.sizes[name]]
+
+    def positions(self, name):
+        """How many rows of its sequence were pushed before each row, int32 [batch, heads, k]; as for :meth:`weights`."""
+        return self._buffers[f"{name}_position"][..., :self.sizes[name]]

@@ -1,0 +1,283 @@
+// mi_cache.hip -- C ABI (include/mi_knn.h) of the 4-bit cache bank: argument checks, launch shapes, workspaces.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/mi_knn.h"
+#include "cache_kernel.h"
+#include "host_common.h"
+
+namespace {
+
+constexpr int64_t MAX_ROWS = (int64_t)1 << 30;
+
+int width_of(int64_t dim)
+{
+    if (dim < 8 || dim > 256 || dim % 8) return 0;
+    return dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+}
+
+int check_cache(const mi_cache_t *c, const char *who)
+{
+    if (!c) return fail(MI_ERR_ARG, "%s: null cache", who);
+    if (!c->key || !c->key_scale || !c->value || !c->value_scale || !c->weight || !c->position || !c->length || !c->seen)
+        return fail(MI_ERR_ARG, "%s: null pointer in the cache", who);
+    if (((uintptr_t)c->key | (uintptr_t)c->key_scale | (uintptr_t)c->value | (uintptr_t)c->value_scale | (uintptr_t)c->weight | (uintptr_t)c->position) & 15)
+        return fail(MI_ERR_ARG, "%s: the cache's buffers must be 16-byte aligned", who);
+    if (c->batch < 1 || c->heads < 1 || c->batch * c->heads > (1 << 24) || c->batch > (1 << 24) || c->heads > (1 << 24))
+        return fail(MI_ERR_ARG, "%s: bad shape batch=%lld heads=%lld", who, (long long)c->batch, (long long)c->heads);
+    if (!width_of(c->dim)) return fail(MI_ERR_UNSUPPORTED, "%s: dim=%lld must be a multiple of 8 in [8, 256]", who, (long long)c->dim);
+    if (c->limit < 1 || c->rows < c->limit || c->rows % 64 || c->rows > MAX_ROWS)
+        return fail(MI_ERR_ARG, "%s: bad capacity rows=%lld limit=%lld", who, (long long)c->rows, (long long)c->limit);
+    return MI_OK;
+}
+
+mi::CacheView view(const mi_cache_t *c)
+{
+    mi::CacheView v{};
+    v.key = c->key, v.key_scale = c->key_scale, v.value = c->value, v.value_scale = c->value_scale;
+    v.weight = c->weight, v.position = c->position, v.length = c->length, v.seen = c->seen;
+    v.batch = (int)c->batch, v.heads = (int)c->heads, v.dim = (int)c->dim, v.rows = (int)c->rows, v.limit = (int)c->limit;
+    return v;
+}
+
+// Byte strides of a [sequence][head][row][dim] tensor; every row has to start on 16 bytes.
+int check_rows(const char *who, const char *what, const void *p, const int64_t *strides, int dtype, long long (&out)[3])
+{
+    if (!p || !strides) return fail(MI_ERR_ARG, "%s: null %s", who, what);
+    const int64_t es = dtype == MI_F32 ? 4 : 2;
+    if ((uintptr_t)p & 15) return fail(MI_ERR_ARG, "%s: %s must be 16-byte aligned", who, what);
+    for (int i = 0; i < 3; ++i) {
+        if (strides[i] < 0 || strides[i] * es % 16) return fail(MI_ERR_ARG, "%s: strides of %s must be multiples of 16 bytes", who, what);
+        out[i] = strides[i] * es;
+    }
+    return MI_OK;
+}
+
+#define MI_TRY(expr)            \
+    do {                        \
+        const int rc_ = (expr); \
+        if (rc_) return rc_;    \
+    } while (0)
+
+int check_grid(const char *who, int64_t blocks)
+{
+    return blocks > INT32_MAX ? fail(MI_ERR_UNSUPPORTED, "%s: too many rows for one launch", who) : (int)MI_OK;
+}
+
+// Launch shape of the attention: tiles of 16 MT query rows, and pieces of the bank's rows so that the card is filled when
+// there are few of them.
+struct AttendPlan {
+    int64_t R, mt, tiles, nsplit;
+    size_t off_ml, off_lse, total;
+};
+
+AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
+{
+    AttendPlan a{};
+    a.R = T * group;
+    a.mt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+    const int64_t wide = (width_of(c->dim) == 256 ? 2 : 4) / (dtype == MI_F32 ? 2 : 1);      // what the register file holds
+    if (a.mt > wide) a.mt = wide;
+    a.tiles = ceil_div(a.R, 16 * a.mt);
+    const int64_t groups = c->batch * c->heads * a.tiles;
+    span = span < 1 ? 1 : span > c->limit ? c->limit : span;
+    int64_t ns = ceil_div(2048, groups);
+    const int64_t most = ceil_div(span, 256);
+    a.nsplit = ns < 1 ? 1 : ns > most ? most : ns;
+    const int64_t rows = c->batch * c->heads * a.R;
+    size_t at = 0;
+    if (a.nsplit > 1) {
+        at = (size_t)(a.nsplit * rows * width_of(c->dim) * 4);
+        a.off_ml = at;
+        at += (size_t)round_up(a.nsplit * rows * 8, 256);
+    }
+    a.off_lse = at;
+    if (accumulate) at += (size_t)round_up(rows * 4, 256);
+    a.total = at < 256 ? 256 : at;
+    return a;
+}
+
+template <int DT, int NB>
+hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, int64_t chunks, hipStream_t s)
+{
+    const int64_t bh = (int64_t)p.c.batch * p.c.heads;
+    const dim3 grid((unsigned)(bh * a.tiles * a.nsplit));
+    if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
+    if constexpr (NB < 8 || DT != mi::CACHE_F32)
+        if (a.mt == 2) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 2>), grid, dim3(256), 0, s, p);
+    if constexpr (NB < 8 && DT != mi::CACHE_F32)
+        if (a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
+    if (a.nsplit > 1)
+        hipLaunchKernelGGL((mi::cache_join_kernel<DT, 32 * NB>), dim3((unsigned)ceil_div(bh * a.R * (4 * NB), 256)), dim3(256), 0, s, p);
+    if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * chunks)), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_attend_w(int width, const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, int64_t chunks, hipStream_t s)
+{
+    return width == 64 ? launch_attend<DT, 2>(p, a, accumulate, chunks, s) : width == 128 ? launch_attend<DT, 4>(p, a, accumulate, chunks, s)
+                                                                                         : launch_attend<DT, 8>(p, a, accumulate, chunks, s);
+}
+
+template <int DT>
+void launch_push(int width, const mi::PushParams &p, hipStream_t s)
+{
+    const dim3 grid((unsigned)ceil_div((int64_t)p.c.batch * p.c.heads * p.T * (width / 4), 256));
+    if (width == 64) hipLaunchKernelGGL((mi::cache_push_kernel<DT, 64>), grid, dim3(256), 0, s, p);
+    else if (width == 128) hipLaunchKernelGGL((mi::cache_push_kernel<DT, 128>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((mi::cache_push_kernel<DT, 256>), grid, dim3(256), 0, s, p);
+}
+
+bool known_dtype(int dtype) { return dtype == MI_F32 || dtype == MI_BF16 || dtype == MI_F16; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t mi_cache_width(int64_t dim) { return width_of(dim); }
+
+int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_strides, const void *value, const int64_t *value_strides,
+                  int dtype, int64_t T, const int32_t *counts, void *held_key, void *held_value, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_push"));
+    if (!known_dtype(dtype)) return fail(MI_ERR_ARG, "mi_cache_push: unknown dtype %d", dtype);
+    if (T < 0 || T > MAX_ROWS) return fail(MI_ERR_ARG, "mi_cache_push: bad T=%lld", (long long)T);
+    if (!held_key != !held_value) return fail(MI_ERR_ARG, "mi_cache_push: held_key and held_value go together");
+    if (((uintptr_t)held_key | (uintptr_t)held_value) & 15) return fail(MI_ERR_ARG, "mi_cache_push: held rows must be 16-byte aligned");
+    if (T == 0) return MI_OK;
+    mi::PushParams p{};
+    MI_TRY(check_rows("mi_cache_push", "key", key, key_strides, dtype, p.key_s));
+    MI_TRY(check_rows("mi_cache_push", "value", value, value_strides, dtype, p.value_s));
+    const int width = width_of(cache->dim);
+    MI_TRY(check_grid("mi_cache_push", ceil_div(cache->batch * cache->heads * T * (width / 4), 256)));
+    p.c = view(cache);
+    p.key = (const char *)key, p.value = (const char *)value;
+    p.counts = counts;
+    p.T = (int)T;
+    p.held_key = (char *)held_key, p.held_value = (char *)held_value;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == MI_F32) launch_push<mi::CACHE_F32>(width, p, s);
+    else if (dtype == MI_BF16) launch_push<mi::CACHE_BF16>(width, p, s);
+    else launch_push<mi::CACHE_F16>(width, p, s);
+    HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(mi::cache_advance_kernel, dim3((unsigned)ceil_div(cache->batch, 64)), dim3(64), 0, s, p);
+    HIP_CHECK(hipGetLastError());
+    return MI_OK;
+}
+
+int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t length, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_trim"));
+    if (!lengths && (length < 0 || length > INT32_MAX)) return fail(MI_ERR_ARG, "mi_cache_trim: bad length %lld", (long long)length);
+    hipLaunchKernelGGL(mi::cache_trim_kernel, dim3((unsigned)ceil_div(cache->batch, 64)), dim3(64), 0, (hipStream_t)stream, view(cache), lengths, (int)length);
+    HIP_CHECK(hipGetLastError());
+    return MI_OK;
+}
+
+int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_read"));
+    if (!key || !value || (((uintptr_t)key | (uintptr_t)value) & 15)) return fail(MI_ERR_ARG, "mi_cache_read: key and value must be 16-byte aligned");
+    const int width = width_of(cache->dim);
+    const int64_t blocks = ceil_div(cache->batch * cache->heads * cache->limit * (width / 4), 256);
+    MI_TRY(check_grid("mi_cache_read", blocks));
+    const dim3 grid((unsigned)blocks);
+    hipStream_t s = (hipStream_t)stream;
+    const mi::CacheView v = view(cache);
+    if (width == 64) hipLaunchKernelGGL(mi::cache_read_kernel<64>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
+    else if (width == 128) hipLaunchKernelGGL(mi::cache_read_kernel<128>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
+    else hipLaunchKernelGGL(mi::cache_read_kernel<256>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
+    HIP_CHECK(hipGetLastError());
+    return MI_OK;
+}
+
+size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
+{
+    if (check_cache(cache, "mi_cache_attend_workspace_bytes") || !known_dtype(dtype) || T < 1 || group < 1 || group > 65536 || T > MAX_ROWS / group) return 0;
+    return attend_plan(cache, dtype, T, group, span, accumulate).total;
+}
+
+int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *query_strides, void *out, const int64_t *out_strides,
+                    int dtype, int64_t T, int64_t group, const int32_t *counts, float scale, int causal, int accumulate, int64_t span,
+                    void *workspace, size_t workspace_bytes, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_attend"));
+    if (!known_dtype(dtype)) return fail(MI_ERR_ARG, "mi_cache_attend: unknown dtype %d", dtype);
+    if (T < 0 || group < 1 || group > 65536 || T > MAX_ROWS / group) return fail(MI_ERR_ARG, "mi_cache_attend: bad shape T=%lld group=%lld", (long long)T, (long long)group);
+    if (!(scale > 0.f) || !isfinite(scale)) return fail(MI_ERR_ARG, "mi_cache_attend: scale must be positive and finite");
+    if (T == 0) return MI_OK;
+    mi::CacheAttendParams p{};
+    MI_TRY(check_rows("mi_cache_attend", "query", query, query_strides, dtype, p.q_s));
+    MI_TRY(check_rows("mi_cache_attend", "out", out, out_strides, dtype, p.out_s));
+    const AttendPlan a = attend_plan(cache, dtype, T, group, span, accumulate);
+    if (!workspace || ((uintptr_t)workspace & 15)) return fail(MI_ERR_ARG, "mi_cache_attend: workspace must be 16-byte aligned");
+    if (workspace_bytes < a.total) return fail(MI_ERR_WORKSPACE, "mi_cache_attend: workspace %zu < required %zu", workspace_bytes, a.total);
+    const int width = width_of(cache->dim);
+    const int64_t bh = cache->batch * cache->heads;
+    const int64_t chunks = ceil_div(span < 1 ? 1 : span > cache->limit ? cache->limit : span, 128);
+    MI_TRY(check_grid("mi_cache_attend", bh * a.tiles * a.nsplit));
+    MI_TRY(check_grid("mi_cache_attend", ceil_div(bh * a.R * (width / 8), 256)));
+    MI_TRY(check_grid("mi_cache_attend", bh * chunks));
+    p.c = view(cache);
+    p.q = (const char *)query;
+    p.out = (char *)out;
+    p.counts = counts;
+    p.T = (int)T, p.G = (int)group, p.causal = causal ? 1 : 0;
+    p.R = (int)a.R, p.tiles = (int)a.tiles, p.nsplit = (int)a.nsplit, p.chunks = (int)chunks;
+    p.c2 = scale * mi::CACHE_LOG2E;
+    p.part = (float *)workspace;
+    p.part_ml = (float2 *)((char *)workspace + a.off_ml);
+    p.lse = accumulate ? (float *)((char *)workspace + a.off_lse) : nullptr;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == MI_F32) HIP_CHECK(launch_attend_w<mi::CACHE_F32>(width, p, a, accumulate, chunks, s));
+    else if (dtype == MI_BF16) HIP_CHECK(launch_attend_w<mi::CACHE_BF16>(width, p, a, accumulate, chunks, s));
+    else HIP_CHECK(launch_attend_w<mi::CACHE_F16>(width, p, a, accumulate, chunks, s));
+    return MI_OK;
+}
+
+size_t mi_cache_evict_workspace_bytes(const mi_cache_t *cache, int64_t keep)
+{
+    if (check_cache(cache, "mi_cache_evict_workspace_bytes") || keep < 1) return 0;
+    return (size_t)(round_up(cache->batch * cache->heads * 4, 256) + cache->batch * cache->heads * keep * 8);
+}
+
+int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent,
+                   void *workspace, size_t workspace_bytes, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_evict"));
+    if (into && into != cache) {
+        MI_TRY(check_cache(into, "mi_cache_evict"));
+        if (into->batch != cache->batch || into->heads != cache->heads || into->dim != cache->dim) return fail(MI_ERR_ARG, "mi_cache_evict: the two banks differ in batch, heads or dim");
+        if (into->key == cache->key || into->length == cache->length) return fail(MI_ERR_ARG, "mi_cache_evict: the two banks share memory");
+    } else into = cache;
+    if (keep < 1 || keep > into->limit) return fail(MI_ERR_ARG, "mi_cache_evict: keep=%lld outside [1, %lld]", (long long)keep, (long long)into->limit);
+    if (recent < 0 || recent > keep) return fail(MI_ERR_ARG, "mi_cache_evict: recent=%lld outside [0, keep=%lld]", (long long)recent, (long long)keep);
+    if (!workspace || ((uintptr_t)workspace & 15)) return fail(MI_ERR_ARG, "mi_cache_evict: workspace must be 16-byte aligned");
+    const size_t need = mi_cache_evict_workspace_bytes(cache, keep);
+    if (workspace_bytes < need) return fail(MI_ERR_WORKSPACE, "mi_cache_evict: workspace %zu < required %zu", workspace_bytes, need);
+    const int64_t bh = cache->batch * cache->heads;
+    const int width = width_of(cache->dim);
+    mi::EvictParams p{};
+    p.c = view(cache), p.into = view(into);
+    p.keep = (int)keep, p.recent = (int)recent, p.in_place = into == cache;
+    p.count = (int *)workspace;
+    p.pairs = (int2 *)((char *)workspace + round_up(bh * 4, 256));
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(mi::cache_select_kernel, dim3((unsigned)bh), dim3(mi::EVICT_THREADS), 0, s, p);
+    HIP_CHECK(hipGetLastError());
+    // a workgroup copies 2048 / width rows a turn; as many of them as the card holds at once are enough
+    const int64_t turn = 2048 / width;
+    int64_t chunks = ceil_div(keep, turn);
+    const int64_t fill = ceil_div(4096, bh);
+    if (chunks > fill) chunks = fill;
+    const dim3 grid((unsigned)(bh * chunks));
+    if (width == 64) hipLaunchKernelGGL(mi::cache_move_kernel<64>, grid, dim3(256), 0, s, p, (int)chunks);
+    else if (width == 128) hipLaunchKernelGGL(mi::cache_move_kernel<128>, grid, dim3(256), 0, s, p, (int)chunks);
+    else hipLaunchKernelGGL(mi::cache_move_kernel<256>, grid, dim3(256), 0, s, p, (int)chunks);
+    HIP_CHECK(hipGetLastError());
+    return MI_OK;
+}
+
+}  // extern "C"

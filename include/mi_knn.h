@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MI_ABI_VERSION 8
+#define MI_ABI_VERSION 9
 
 enum { MI_OK = 0, MI_ERR_ARG = -1, MI_ERR_HIP = -2, MI_ERR_WORKSPACE = -3, MI_ERR_UNSUPPORTED = -4 };
 enum { MI_F32 = 0, MI_BF16 = 1 };            /* compute dtype of the similarity GEMM            */
@@ -223,6 +223,63 @@ int mi_soft_knn(const float *feature, const float *bank_feature, const float *ba
  * (models/memory_bank.py:65-72). */
 int mi_queue_push_stash(void *queue, int64_t K, int64_t row_bytes, int64_t ptr,
                         const void *value, int64_t b, void *stash, int64_t *new_ptr, mi_stream_t stream);
+
+/* ---- A bank of key / value rows held in 4 bits (no reference counterpart: its banks, models/memory_bank.py, hold whole
+ * numbers of bytes, are read by dense products, and drop their oldest rows).  Rows of `heads` heads for `batch` sequences:
+ * appended quantised (push), read by softmax attention (attend), dropped by the attention they got (evict).
+ *
+ * Format: a row of `dim` values, zero padded to `width` = 64, 128 or 256, in blocks of 32.  A block has one scale 2^e, e the
+ * smallest integer with max|x| <= 7 * 2^e, clamped to [-126, 125], held as the byte e + 127; elements are x / 2^e rounded to
+ * nearest (ties to even, saturating) on 0 0.5 1 1.5 2 3 4 6 with a sign bit, two a byte, the even one in the low four bits.
+ * A row of a head with a NaN or an infinity in its key or its value is held as NaN whole (all scale bytes 255, elements 0).
+ * All pointers are device memory, 16-byte aligned; `rows` (allocated) is a multiple of 64, `limit` <= rows the most in use. */
+typedef struct {
+    uint8_t *key, *key_scale;        /* [batch][heads][rows][width / 2], [batch][heads][width / 32][rows] */
+    uint8_t *value, *value_scale;
+    float *weight;                   /* [batch][heads][rows]: attention that each row got since its push */
+    int32_t *position;               /* [batch][heads][rows]: how many rows of its sequence were pushed before it */
+    int32_t *length, *seen;          /* [batch]: rows in use, rows pushed so far */
+    int64_t batch, heads, dim, rows, limit;
+} mi_cache_t;
+enum { MI_F16 = 2 };                         /* besides MI_F32, MI_BF16: types of keys, values and queries */
+
+/* Width that a row of `dim` values is held at (dim % 8 == 0, 8 <= dim <= 256), or 0. */
+int64_t mi_cache_width(int64_t dim);
+
+/* Appends T rows behind the last row of every sequence, or the first counts[b] of them (counts: device int32[batch] or NULL;
+ * taken as 0 .. T).  key, value: [batch][heads][T][dim] of `dtype`, strides in ELEMENTS for sequence, head and row (multiples of
+ * 8 elements and 16-byte aligned rows); dims are contiguous.  Rows beyond `limit` are dropped.  The weight of a new row is 0.
+ * held_key, held_value (contiguous [batch][heads][T][dim] of `dtype`, both or neither): the values that the bank now holds;
+ * zeros for rows that were not stored. */
+int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_strides, const void *value, const int64_t *value_strides,
+                  int dtype, int64_t T, const int32_t *counts, void *held_key, void *held_value, mi_stream_t stream);
+
+/* length[b] = min(length[b], lengths[b]) (device int32[batch]; NULL: `length` for all); positions go on from the cut. */
+int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t length, mi_stream_t stream);
+
+/* Rows [0, limit) as bf16 (exact), [batch][heads][limit][dim] each; rows that are not in use are zeros. */
+int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t stream);
+
+/* Softmax attention of T query rows of heads * group query heads over the bank; query head h reads head h / group.
+ *   out[b, h, t] = sum_s p[s] value[s],  p = softmax over the visible slots s of scale * query[b, h, t] . key[s]
+ * Row t of sequence b is real if t < counts[b] (NULL: all T).  causal: the last counts[b] rows of the sequence are the query rows
+ * themselves, so row t sees the slots before length[b] - counts[b] + t + 1; otherwise all of length[b].  A row that is not real
+ * or sees nothing gives zeros.  accumulate: weight[b, h, s] += the sum of p[s] over the real rows and the group's heads.
+ * query, out: [batch][heads * group][T][dim] of `dtype` with strides as in mi_cache_push.  Products are exact in bf16 pieces of
+ * the query (one for bf16, two for float16, three for float32), sums and softmax statistics are float32.
+ * `span`: about how many rows are in use (it sizes the launch; the result is right for any span >= 1). */
+size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int accumulate);
+int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *query_strides, void *out, const int64_t *out_strides,
+                    int dtype, int64_t T, int64_t group, const int32_t *counts, float scale, int causal, int accumulate, int64_t span,
+                    void *workspace, size_t workspace_bytes, mi_stream_t stream);
+
+/* Keeps `keep` rows of every (sequence, head) that has more: those pushed among the last `recent` of the sequence, then those
+ * with the largest weight (NaN counts as the largest), ties to the lower slot.  Slots below `keep` whose row leaves take, in
+ * ascending order, the kept rows of the slots from `keep` on.  into == cache: in place.  Otherwise `into` (same batch, heads and
+ * dim; limit >= keep) receives the rows that are kept and `cache` is left as it was.  0 <= recent <= keep. */
+size_t mi_cache_evict_workspace_bytes(const mi_cache_t *cache, int64_t keep);
+int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent,
+                   void *workspace, size_t workspace_bytes, mi_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -64,5 +64,5 @@ for name, edits in (("e_base", []), ("e_halfreads", HALF), ("e_l2all", L2ALL), (
         open(h, "w").write(hs.replace(NOSPEC_OLD, NOSPEC_NEW))
         out = os.path.join(PKG, f"libmi_knn_{name}.so")
         subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC",
-                               "-o", out, "mi_knn.hip"], cwd=os.path.join(d, "pkg", "csrc"))
+                               "-o", out, "mi_knn.hip", "mi_cache.hip"], cwd=os.path.join(d, "pkg", "csrc"))
         print(out)

@@ -53,5 +53,5 @@ for name, new in NEW.items():
         open(h, "w").write(hs.replace(nospec, nospec.replace("if (N >", "if (false && N >")))
         out = os.path.join(PKG, f"libmi_knn_{name}.so")
         subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC",
-                               "-o", out, "mi_knn.hip"], cwd=os.path.join(d, "pkg", "csrc"))
+                               "-o", out, "mi_knn.hip", "mi_cache.hip"], cwd=os.path.join(d, "pkg", "csrc"))
         print(out)

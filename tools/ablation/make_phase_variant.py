@@ -61,5 +61,5 @@ with tempfile.TemporaryDirectory() as d:
     open(p, "w").write(s)
     out = os.path.join(PKG, "libmi_knn_phase%s.so" % (sys.argv[1] if len(sys.argv) > 1 else ""))
     subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC"]
-                          + sys.argv[2:] + ["-o", out, "mi_knn.hip"], cwd=os.path.join(d, "pkg", "csrc"))
+                          + sys.argv[2:] + ["-o", out, "mi_knn.hip", "mi_cache.hip"], cwd=os.path.join(d, "pkg", "csrc"))
     print(out)

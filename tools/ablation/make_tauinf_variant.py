@@ -37,5 +37,5 @@ with tempfile.TemporaryDirectory() as d:
     open(p, "w").write(s)
     out = os.path.join(PKG, "libmi_knn_tauinf%s.so" % suffix)
     subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC",
-                           "-o", out, "mi_knn.hip"], cwd=os.path.join(d, "pkg", "csrc"))
+                           "-o", out, "mi_knn.hip", "mi_cache.hip"], cwd=os.path.join(d, "pkg", "csrc"))
     print(out)
