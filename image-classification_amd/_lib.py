@@ -103,7 +103,7 @@ def lib() -> ctypes.CDLL:
     L.mi_cache_evict_workspace_bytes.restype = sz
     L.mi_cache_evict_workspace_bytes.argtypes = [cache, i64]
     L.mi_cache_evict.restype = i32
-    L.mi_cache_evict.argtypes = [cache, cache, i64, i64, p, sz, p]
+    L.mi_cache_evict.argtypes = [cache, cache, i64, i64, i64, p, sz, p]
     if L.mi_abi_version() != ABI_VERSION:
         raise MiKnnError(f"libmi_knn.so ABI {L.mi_abi_version()} != expected {ABI_VERSION}: rebuild")
     _lib = L

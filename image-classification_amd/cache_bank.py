@@ -241,7 +241,8 @@ class CacheBank(nn.Module):
         with _on(device):
             self._changes(target)
             ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(ctypes.byref(view), keep)), dtype=torch.uint8, device=device)
-            _lib.check(L.mi_cache_evict(ctypes.byref(view), ctypes.byref(other), keep, recent, ws.data_ptr(), ws.numel(),
+            span = max(1, self.sizes[name] if name in self._captured else self._bounds[name])
+            _lib.check(L.mi_cache_evict(ctypes.byref(view), ctypes.byref(other), keep, recent, span, ws.data_ptr(), ws.numel(),
                                         _lib.stream_ptr(device)), "mi_cache_evict")
         self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bounds[name]))
 

@@ -261,6 +261,7 @@ struct CacheAttendParams {
     float2 *part_ml;                         //             ... and [split][batch heads][R] (maximum, sum), maximum in log2 units
     int chunks;                              // weights: workgroups a (sequence, head), each takes every chunks-th 128 rows
     float *lse;                              // [batch heads][R] log2 of the softmax denominator (weights wanted), or null
+    float *scores;                           // [batch heads][R][rows] scores before the scale (few query rows, weights wanted), or null
 };
 
 // How many slots a query row sees: the last n rows of a sequence are the n query rows themselves when `causal`.
@@ -471,19 +472,22 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
     const int first = split * per, last = min(units, first + per);
 
     cf32x4 o[MT][2 * NB];
-    float mx[MT], sum[MT];
+    float mx[MT], ref[MT], sum[MT];          // maximum, its share of the exponent, sum of this lane's probabilities
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         mx[m] = -INFINITY;
+        ref[m] = 0.f;
         sum[m] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) o[m][i] = cf32x4{0, 0, 0, 0};
     }
     const UnitAt<NB> at(p.c, bh, lane);
+    Unit<NB> next;
+    if (first + wave < last) at.load((first + wave) * 32, next);
     for (int un = first + wave; un < last; un += 4) {
         const int u0 = un * 32;
-        Unit<NB> u;
-        at.load(u0, u);
+        const Unit<NB> u = next;
+        at.load(min(un + 4, last - 1) * 32, next);        // the next unit is on its way while this one is computed
         cf32x4 s[MT][2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
@@ -506,23 +510,29 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
                 for (int e = 0; e < 8; ++e)
                     if (u0 + 16 * (e >> 2) + 4 * j + (e & 3) >= lim[m]) s[m][e >> 2][e & 3] = -INFINITY;
             }
+            if (p.scores && c < p.R) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) *(cf32x4 *)(p.scores + (bh * p.R + c) * p.c.rows + u0 + 16 * a + 4 * j) = s[m][a];
+            }
             float top = s[m][0][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) top = fmaxf(top, s[m][e >> 2][e & 3]);
-            const float now = fmaxf(mx[m], across_j_max(top));
-            const float ref = now == -INFINITY ? 0.f : now * p.c2;
-            const float shrink = __builtin_amdgcn_exp2f(fmaf(mx[m], p.c2, -ref));
-            mx[m] = now;
-            float x[8], part = 0.f;
+            if (__any(top > mx[m])) {                     // after the first units the maximum hardly ever moves
+                const float now = fmaxf(mx[m], across_j_max(top));
+                ref[m] = now == -INFINITY ? 0.f : now * p.c2;
+                const float shrink = __builtin_amdgcn_exp2f(fmaf(mx[m], p.c2, -ref[m]));
+                mx[m] = now;
+                sum[m] *= shrink;
+#pragma unroll
+                for (int i = 0; i < 2 * NB; ++i) o[m][i] *= shrink;
+            }
+            float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], p.c2, -ref));
-                part += x[e];
+                x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], p.c2, -ref[m]));
+                sum[m] += x[e];
             }
-            sum[m] = sum[m] * shrink + part;
             split_pieces<PP>(x, pf[m]);
-#pragma unroll
-            for (int i = 0; i < 2 * NB; ++i) o[m][i] *= shrink;
         }
 #pragma unroll
         for (int i2 = 0; i2 < NB; ++i2) {                 // channels 2 i2, 2 i2 + 1 of each lane
@@ -562,8 +572,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
         float top = s_m[0][c];
 #pragma unroll
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][c]);
-        const float ref = top == -INFINITY ? 0.f : top * p.c2;
-        const float f = __builtin_amdgcn_exp2f(fmaf(mx[m], p.c2, -ref));
+        const float f = __builtin_amdgcn_exp2f(fmaf(mx[m], p.c2, top == -INFINITY ? 0.f : -(top * p.c2)));
         // channel of o[i][r]: (4 j + r) * 2 NB + i: 2 NB neighbours for each r
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -596,27 +605,58 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
     }
 }
 
-// Joins the pieces of a row: W / 8 lanes a row, 8 channels a lane.
+// Joins the pieces of a row, one workgroup a row: W / 8 lanes side by side in a piece, 2048 / W pieces at a time.  (One lane
+// group a row, walking over the pieces, took 152 us for 256 pieces of 32 rows: a chain of dependent loads.)
+constexpr int CACHE_MAX_SPLIT = 256;
+
 template <int DT, int W>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p)
 {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long all = (long long)p.c.batch * p.c.heads * p.R, g0 = at / (W / 8);
-    const int d = (int)(at % (W / 8)) * 8;
-    if (g0 >= all) return;
+    constexpr int LANES = W / 8, GROUPS = 256 / LANES;
+    __shared__ float s_f[CACHE_MAX_SPLIT];
+    __shared__ float s_x[GROUPS][W];
+    const long long all = (long long)p.c.batch * p.c.heads * p.R, g0 = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, d = tid % LANES * 8, group = tid / LANES;
+    // every wave finds the maximum and the denominator for itself
+    float2 ml[CACHE_MAX_SPLIT / 64];
     float big = -INFINITY;
-    for (int s = 0; s < p.nsplit; ++s) big = fmaxf(big, p.part_ml[s * all + g0].x);
-    float den = 0.f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float2 ml = p.part_ml[s * all + g0];
-        if (ml.x == -INFINITY) continue;                  // nothing seen there: its sums may be left unread
-        const float f = __builtin_amdgcn_exp2f(ml.x - big);
-        den += ml.y * f;
+#pragma unroll
+    for (int k = 0; k < CACHE_MAX_SPLIT / 64; ++k) {
+        const int s = k * 64 + lane;
+        ml[k] = s < p.nsplit ? p.part_ml[s * all + g0] : make_float2(-INFINITY, 0.f);
+        big = fmaxf(big, ml[k].x);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) big = fmaxf(big, __shfl_xor(big, m));
+    float den = 0.f;
+#pragma unroll
+    for (int k = 0; k < CACHE_MAX_SPLIT / 64; ++k) {
+        // a piece that saw nothing has no sums to read
+        const float f = ml[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - big);
+        den += ml[k].y * f;
+        if (tid < 64) s_f[k * 64 + lane] = ml[k].x == -INFINITY ? -1.f : f;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) den += __shfl_xor(den, m);
+    __syncthreads();
+    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = group; s < p.nsplit; s += GROUPS) {
+        const float f = s_f[s];
+        if (f < 0.f) continue;                            // (a NaN goes on)
         float y[8];
         load8<CACHE_F32>(p.part + (s * all + g0) * W + d, y);
+#pragma unroll
         for (int i = 0; i < 8; ++i) x[i] += y[i] * f;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_x[group][d + i] = x[i];
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < GROUPS && g < p.nsplit; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += s_x[g][d + i];
     const float inv = 1.f / den;
+#pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = big == -INFINITY ? 0.f : x[i] * inv;
     const long long bh = g0 / p.R;
     const int row = (int)(g0 % p.R), b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads), t = row / p.G, g = row - t * p.G;
@@ -675,6 +715,34 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
     }
 }
 
+// The same where the attention kernel left its scores behind: four slots a thread, R scores each.
+__global__ __launch_bounds__(256) void cache_weigh_scores_kernel(CacheAttendParams p)
+{
+    const long long bh = blockIdx.x / p.chunks;
+    const int b = (int)(bh / p.c.heads);
+    int len = p.c.length[b];
+    len = len > p.c.limit ? p.c.limit : len;
+    const int n = real_rows(p.counts, b, p.T);
+    for (int slot = ((int)(blockIdx.x % p.chunks) * 256 + threadIdx.x) * 4; slot < len; slot += p.chunks * 1024) {
+        float w[4] = {0, 0, 0, 0};
+        for (int row = 0; row < p.R; ++row) {
+            const int lim = visible(row / p.G, n, len, p.causal);
+            if (lim <= slot) continue;                    // (scores of a unit that no row of the tile sees were never written)
+            const float lse = p.lse[bh * p.R + row];
+            const cf32x4 s = *(const cf32x4 *)(p.scores + (bh * p.R + row) * p.c.rows + slot);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[e], p.c2, -lse));
+                w[e] += slot + e < lim ? x : 0.f;
+            }
+        }
+        float *to = p.c.weight + bh * p.c.rows + slot;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (slot + e < len) to[e] += w[e];
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------ eviction
 struct EvictParams {
     CacheView c, into;
@@ -692,133 +760,147 @@ __device__ __forceinline__ uint32_t evict_rank(float w, int position, int from)
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_THREADS = 1024, EVICT_BINS = 2048;
+constexpr int EVICT_RESIDENT = 36864;        // ranks of so many rows fit the 160 KB of shared memory beside the histogram
 
-// Exclusive prefix sum over the workgroup of two counts at once; totals in `all`.
-__device__ __forceinline__ int2 block_scan2(int2 v, int2 *s_wave, int2 &all)
+// Exclusive prefix sums of two numbers over the waves of the workgroup (one value a wave, from any lane of it).
+__device__ __forceinline__ int2 wave_scan2(int2 v, int2 *s_wave, int2 &all)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int2 x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int a = __shfl_up(x.x, d), e = __shfl_up(x.y, d);
-        if (lane >= d) x.x += a, x.y += e;
-    }
+    const int wave = threadIdx.x >> 6;
     __syncthreads();
-    if (lane == 63) s_wave[wave] = x;
+    if ((threadIdx.x & 63) == 0) s_wave[wave] = v;
     __syncthreads();
     int2 before = make_int2(0, 0);
     all = make_int2(0, 0);
+#pragma unroll
     for (int i = 0; i < EVICT_THREADS / 64; ++i) {
         if (i < wave) before.x += s_wave[i].x, before.y += s_wave[i].y;
         all.x += s_wave[i].x, all.y += s_wave[i].y;
     }
-    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+    return before;
 }
 
-// One workgroup per (sequence, head): radix select of the keep-th rank, then the lists of what has to be copied.  The freed
-// slots below `keep` take, in ascending order, the kept rows from above it: in place no row is read that another one is
-// written to, and no more rows move than left.
-__global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams p)
+// The rank that the keep-th row has, by digits of 11, 11 and 10 bits, then the lists of what has to be copied: wave w goes over
+// the w-th sixteenth of the slots, 64 neighbours at a time, and counts with ballots.
+template <typename Rank>
+__device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, int n, Rank rank, int *s_hist, int2 *s_wave, int *s_pick)
 {
-    __shared__ int s_hist[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keep = p.keep;
+    int2 *pairs = p.pairs + bh * keep;
+    uint32_t prefix = 0, known = 0;
+    int left = keep;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t mask = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) s_hist[i] = 0;
+        __syncthreads();
+        for (int i0 = wave * 64; i0 < n; i0 += EVICT_THREADS) {
+            const int i = i0 + lane;
+            const uint32_t r = i < n ? rank(i) : 0u;
+            const bool in = i < n && (r & known) == prefix;
+            const int digit = (int)((r >> shift) & mask);
+            // equal neighbours (rows that nothing attended to yet) are counted once for the wave, not 64 times in turn
+            const unsigned long long who = __ballot(in);
+            if (!who) continue;
+            const int first = __builtin_amdgcn_readlane(digit, __ffsll((long long)who) - 1);
+            const unsigned long long same = __ballot(in && digit == first);
+            if (lane == 0) atomicAdd(&s_hist[first], __popcll(same));
+            if (in && digit != first) atomicAdd(&s_hist[digit], 1);
+        }
+        __syncthreads();
+        // the bin that holds the left-th largest: bins from the top, two a thread
+        const int top = EVICT_BINS - 1 - 2 * tid, a = s_hist[top], b = s_hist[top - 1];
+        int sum = a + b;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(sum, d);
+            if (lane >= d) sum += v;
+        }
+        int2 all;
+        const int total = __builtin_amdgcn_readlane(sum, 63);
+        const int above = wave_scan2(make_int2(total, 0), s_wave, all).x + sum - a - b;
+        if (above < left && above + a + b >= left) {
+            const bool second = above + a < left;
+            s_pick[0] = second ? top - 1 : top;
+            s_pick[1] = left - above - (second ? a : 0);
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_pick[0] << shift;
+        left = s_pick[1];
+        known |= mask << shift;
+        __syncthreads();
+    }
+    // rows above the edge stay, and of those on it the `left` lowest slots
+    const uint32_t edge = prefix;
+    const int seg = ((n + EVICT_THREADS - 1) / EVICT_THREADS) * 64, lo = min(n, wave * seg), hi = min(n, lo + seg);
+    const unsigned long long below = (1ull << lane) - 1;
+    int eq = 0;
+    for (int i0 = lo; i0 < hi; i0 += 64) eq += __popcll(__ballot(i0 + lane < hi && rank(i0 + lane) == edge));
+    int2 all;
+    const int eq0 = wave_scan2(make_int2(eq, 0), s_wave, all).x;
+    int2 off = make_int2(0, 0);              // freed slots below keep, kept rows from there on
+    int base = 0;                            // pairs before those of the freed slots
+#pragma unroll
+    for (int write = 0; write < 2; ++write) {
+        int at = eq0, holes = 0, tails = 0;
+        for (int i0 = lo; i0 < hi; i0 += 64) {
+            const int i = i0 + lane;
+            const uint32_t r = i < hi ? rank(i) : 0u;
+            const unsigned long long on = __ballot(i < hi && r == edge);
+            const bool kept = i < hi && (r > edge || (r == edge && at + __popcll(on & below) < left));
+            const bool hole = i < hi && i < keep && !kept, tail = i >= keep && kept;
+            const unsigned long long h = __ballot(hole), t = __ballot(tail);
+            if (write) {
+                const int nh = off.x + holes + __popcll(h & below), nt = off.y + tails + __popcll(t & below);
+                if (hole) pairs[base + nh].x = i;
+                if (tail) pairs[base + nt].y = i;
+                if (base && i < keep && kept) pairs[i - nh] = make_int2(i, i);
+            }
+            at += __popcll(on);
+            holes += __popcll(h);
+            tails += __popcll(t);
+        }
+        if (!write) {
+            off = wave_scan2(make_int2(holes, tails), s_wave, all);
+            base = p.in_place ? 0 : keep - all.x;
+            if (tid == 0) p.count[bh] = p.in_place ? all.x : keep;
+        }
+    }
+}
+
+// One workgroup per (sequence, head).  The freed slots below `keep` take, in ascending order, the kept rows from above: in place
+// no row is read that another one is written to, and no more rows move than left.  Ranks are built in one pass over weights and
+// positions and stay in shared memory where they fit; `resident` of them do.
+__global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams p, int resident)
+{
+    extern __shared__ uint32_t s_rank[];
+    __shared__ int s_hist[EVICT_BINS];
     __shared__ int2 s_wave[EVICT_THREADS / 64];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_left;
+    __shared__ int s_pick[2];
     const long long bh = blockIdx.x;
     const int b = (int)(bh / p.c.heads), tid = threadIdx.x;
     int n = p.c.length[b];
     n = n > p.c.limit ? p.c.limit : n;
-    const int from = p.c.seen[b] - p.recent, keep = p.keep;
-    const float *w = p.c.weight + bh * p.c.rows;
-    const int *pos = p.c.position + bh * p.c.rows;
-    int2 *pairs = p.pairs + bh * keep;
-    if (n <= keep) {
+    if (n <= p.keep) {
         if (!p.in_place)
-            for (int i = tid; i < n; i += EVICT_THREADS) pairs[i] = make_int2(i, i);
+            for (int i = tid; i < n; i += EVICT_THREADS) p.pairs[bh * p.keep + i] = make_int2(i, i);
         if (tid == 0) p.count[bh] = p.in_place ? 0 : n;
         return;
     }
-    if (tid == 0) s_prefix = 0, s_left = keep;
-    uint32_t known = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix;
-        for (int i = tid; i < n; i += EVICT_THREADS) {
-            const uint32_t r = evict_rank(w[i], pos[i], from);
-            if ((r & known) == prefix) atomicAdd(&s_hist[(r >> shift) & 255], 1);
+    const int from = p.c.seen[b] - p.recent;
+    const float *w = p.c.weight + bh * p.c.rows;
+    const int *pos = p.c.position + bh * p.c.rows;
+    if (n <= resident) {
+        for (int i = tid * 4; i < n; i += EVICT_THREADS * 4) {        // rows are allocated in 64s: whole vectors
+            const float4 x = *(const float4 *)(w + i);
+            const int4 y = *(const int4 *)(pos + i);
+            *(uint4 *)(s_rank + i) = make_uint4(evict_rank(x.x, y.x, from), evict_rank(x.y, y.y, from), evict_rank(x.z, y.z, from), evict_rank(x.w, y.w, from));
         }
         __syncthreads();
-        if (tid == 0) {
-            int left = s_left, d = 255;
-            while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-            s_left = left;
-            s_prefix = prefix | ((uint32_t)d << shift);
-        }
-        known |= 255u << shift;
-        __syncthreads();
-    }
-    const uint32_t edge = s_prefix;
-    const int ties = s_left;                 // rows of rank `edge` that stay: the lowest slots
-    const int per = (n + EVICT_THREADS - 1) / EVICT_THREADS, lo = min(n, tid * per), hi = min(n, lo + per);
-    int eq = 0;
-    for (int i = lo; i < hi; ++i) eq += evict_rank(w[i], pos[i], from) == edge;
-    int2 all;
-    const int before = block_scan2(make_int2(eq, 0), s_wave, all).x;
-    int2 mine = make_int2(0, 0);             // (freed slots below keep, kept rows above it)
-    int at = before;
-    for (int i = lo; i < hi; ++i) {
-        const uint32_t r = evict_rank(w[i], pos[i], from);
-        const bool kept = r > edge || (r == edge && at++ < ties);
-        if (i < keep) mine.x += !kept;
-        else mine.y += kept;
-    }
-    int2 off = block_scan2(mine, s_wave, all);
-    if (tid == 0) p.count[bh] = p.in_place ? all.x : keep;
-    at = before;
-    // in place: pair i = (i-th freed slot, i-th kept row above); otherwise pair s = (s, its source), via the free tail of the
-    // list: the kept rows above are first written where only freed slots are looked up, so they go through shared memory
-    for (int i = lo; i < hi; ++i) {
-        const uint32_t r = evict_rank(w[i], pos[i], from);
-        const bool kept = r > edge || (r == edge && at++ < ties);
-        if (p.in_place) {
-            if (i < keep) {
-                if (!kept) pairs[off.x++].x = i;
-            } else if (kept) pairs[off.y++].y = i;
-        } else if (i < keep) {
-            pairs[i].x = i;
-            if (kept) pairs[i].y = i;
-        }
-    }
-    if (p.in_place) return;
-    // the i-th freed slot of all: its owner waits for the i-th kept row above, in rounds of one list in shared memory
-    __shared__ int s_src[4096];
-    const int2 total = all;
-    for (int base = 0; base < total.x; base += 4096) {
-        __syncthreads();
-        int y = off.y;
-        at = before;
-        for (int i = lo; i < hi; ++i) {
-            const uint32_t r = evict_rank(w[i], pos[i], from);
-            const bool kept = r > edge || (r == edge && at++ < ties);
-            if (i >= keep && kept) {
-                if (y >= base && y < base + 4096) s_src[y - base] = i;
-                ++y;
-            }
-        }
-        __syncthreads();
-        int x = off.x;
-        at = before;
-        for (int i = lo; i < hi && i < keep; ++i) {
-            const uint32_t r = evict_rank(w[i], pos[i], from);
-            const bool kept = r > edge || (r == edge && at++ < ties);
-            if (!kept) {
-                if (x >= base && x < base + 4096) pairs[i].y = s_src[x - base];
-                ++x;
-            }
-        }
-    }
+        select_rows(p, bh, n, [&](int i) { return s_rank[i]; }, s_hist, s_wave, s_pick);
+    } else
+        select_rows(p, bh, n, [&](int i) { return evict_rank(w[i], pos[i], from); }, s_hist, s_wave, s_pick);
 }
 
 // Copies the rows of the lists.  W / 8 lanes a row: a quarter of them for each of key, value, their scales; 16 bytes a lane.

@@ -3,6 +3,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/mi_knn.h"
 #include "cache_kernel.h"
 #include "host_common.h"
@@ -69,7 +71,9 @@ int check_grid(const char *who, int64_t blocks)
 // there are few of them.
 struct AttendPlan {
     int64_t R, mt, tiles, nsplit;
-    size_t off_ml, off_lse, total;
+    int64_t chunks;                          // weights: workgroups a (sequence, head)
+    bool scores;                             // weights: from scores left behind, not from a second product
+    size_t off_ml, off_lse, off_scores, total;
 };
 
 AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
@@ -82,8 +86,8 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     a.tiles = ceil_div(a.R, 16 * a.mt);
     const int64_t groups = c->batch * c->heads * a.tiles;
     span = span < 1 ? 1 : span > c->limit ? c->limit : span;
-    int64_t ns = ceil_div(2048, groups);
-    const int64_t most = ceil_div(span, 256);
+    int64_t ns = ceil_div(768, groups);
+    const int64_t most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
     a.nsplit = ns < 1 ? 1 : ns > most ? most : ns;
     const int64_t rows = c->batch * c->heads * a.R;
     size_t at = 0;
@@ -94,12 +98,19 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     }
     a.off_lse = at;
     if (accumulate) at += (size_t)round_up(rows * 4, 256);
+    // A slot's attention sum costs 8 R bytes if its scores are written and read again, or its key, W / 2 + W / 32 bytes, and the
+    // product once more.  Scores are laid out by the capacity (a captured call may see longer sequences than `span`).
+    const int64_t score_bytes = rows * c->rows * 4;
+    a.scores = accumulate && a.mt == 1 && 8 * a.R <= width_of(c->dim) / 2 && score_bytes <= ((int64_t)1 << 30);
+    a.chunks = ceil_div(span, a.scores ? 1024 : 128);
+    a.off_scores = at;
+    if (a.scores) at += (size_t)score_bytes;
     a.total = at < 256 ? 256 : at;
     return a;
 }
 
 template <int DT, int NB>
-hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, int64_t chunks, hipStream_t s)
+hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, hipStream_t s)
 {
     const int64_t bh = (int64_t)p.c.batch * p.c.heads;
     const dim3 grid((unsigned)(bh * a.tiles * a.nsplit));
@@ -109,16 +120,17 @@ hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, in
     if constexpr (NB < 8 && DT != mi::CACHE_F32)
         if (a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
     if (a.nsplit > 1)
-        hipLaunchKernelGGL((mi::cache_join_kernel<DT, 32 * NB>), dim3((unsigned)ceil_div(bh * a.R * (4 * NB), 256)), dim3(256), 0, s, p);
-    if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * chunks)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((mi::cache_join_kernel<DT, 32 * NB>), dim3((unsigned)(bh * a.R)), dim3(256), 0, s, p);
+    if (a.scores) hipLaunchKernelGGL(mi::cache_weigh_scores_kernel, dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
+    else if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
 template <int DT>
-hipError_t launch_attend_w(int width, const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, int64_t chunks, hipStream_t s)
+hipError_t launch_attend_w(int width, const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, hipStream_t s)
 {
-    return width == 64 ? launch_attend<DT, 2>(p, a, accumulate, chunks, s) : width == 128 ? launch_attend<DT, 4>(p, a, accumulate, chunks, s)
-                                                                                         : launch_attend<DT, 8>(p, a, accumulate, chunks, s);
+    return width == 64 ? launch_attend<DT, 2>(p, a, accumulate, s) : width == 128 ? launch_attend<DT, 4>(p, a, accumulate, s)
+                                                                                         : launch_attend<DT, 8>(p, a, accumulate, s);
 }
 
 template <int DT>
@@ -216,24 +228,24 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     if (workspace_bytes < a.total) return fail(MI_ERR_WORKSPACE, "mi_cache_attend: workspace %zu < required %zu", workspace_bytes, a.total);
     const int width = width_of(cache->dim);
     const int64_t bh = cache->batch * cache->heads;
-    const int64_t chunks = ceil_div(span < 1 ? 1 : span > cache->limit ? cache->limit : span, 128);
     MI_TRY(check_grid("mi_cache_attend", bh * a.tiles * a.nsplit));
-    MI_TRY(check_grid("mi_cache_attend", ceil_div(bh * a.R * (width / 8), 256)));
-    MI_TRY(check_grid("mi_cache_attend", bh * chunks));
+    MI_TRY(check_grid("mi_cache_attend", bh * a.R));
+    MI_TRY(check_grid("mi_cache_attend", bh * a.chunks));
     p.c = view(cache);
     p.q = (const char *)query;
     p.out = (char *)out;
     p.counts = counts;
     p.T = (int)T, p.G = (int)group, p.causal = causal ? 1 : 0;
-    p.R = (int)a.R, p.tiles = (int)a.tiles, p.nsplit = (int)a.nsplit, p.chunks = (int)chunks;
+    p.R = (int)a.R, p.tiles = (int)a.tiles, p.nsplit = (int)a.nsplit, p.chunks = (int)a.chunks;
     p.c2 = scale * mi::CACHE_LOG2E;
     p.part = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + a.off_ml);
+    p.scores = a.scores ? (float *)((char *)workspace + a.off_scores) : nullptr;
     p.lse = accumulate ? (float *)((char *)workspace + a.off_lse) : nullptr;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == MI_F32) HIP_CHECK(launch_attend_w<mi::CACHE_F32>(width, p, a, accumulate, chunks, s));
-    else if (dtype == MI_BF16) HIP_CHECK(launch_attend_w<mi::CACHE_BF16>(width, p, a, accumulate, chunks, s));
-    else HIP_CHECK(launch_attend_w<mi::CACHE_F16>(width, p, a, accumulate, chunks, s));
+    if (dtype == MI_F32) HIP_CHECK(launch_attend_w<mi::CACHE_F32>(width, p, a, accumulate, s));
+    else if (dtype == MI_BF16) HIP_CHECK(launch_attend_w<mi::CACHE_BF16>(width, p, a, accumulate, s));
+    else HIP_CHECK(launch_attend_w<mi::CACHE_F16>(width, p, a, accumulate, s));
     return MI_OK;
 }
 
@@ -243,7 +255,7 @@ size_t mi_cache_evict_workspace_bytes(const mi_cache_t *cache, int64_t keep)
     return (size_t)(round_up(cache->batch * cache->heads * 4, 256) + cache->batch * cache->heads * keep * 8);
 }
 
-int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent,
+int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent, int64_t span,
                    void *workspace, size_t workspace_bytes, mi_stream_t stream)
 {
     MI_TRY(check_cache(cache, "mi_cache_evict"));
@@ -265,7 +277,10 @@ int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep
     p.count = (int *)workspace;
     p.pairs = (int2 *)((char *)workspace + round_up(bh * 4, 256));
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(mi::cache_select_kernel, dim3((unsigned)bh), dim3(mi::EVICT_THREADS), 0, s, p);
+    const int64_t resident = std::min<int64_t>(round_up(span < 1 ? 1 : span > cache->limit ? cache->limit : span, 64), mi::EVICT_RESIDENT);
+    static std::atomic<uint64_t> done{0};
+    HIP_CHECK(ensure_dynamic_lds(mi::cache_select_kernel, (size_t)mi::EVICT_RESIDENT * 4, done));
+    hipLaunchKernelGGL(mi::cache_select_kernel, dim3((unsigned)bh), dim3(mi::EVICT_THREADS), (size_t)resident * 4, s, p, (int)resident);
     HIP_CHECK(hipGetLastError());
     // a workgroup copies 2048 / width rows a turn; as many of them as the card holds at once are enough
     const int64_t turn = 2048 / width;

@@ -276,9 +276,9 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
 /* Keeps `keep` rows of every (sequence, head) that has more: those pushed among the last `recent` of the sequence, then those
  * with the largest weight (NaN counts as the largest), ties to the lower slot.  Slots below `keep` whose row leaves take, in
  * ascending order, the kept rows of the slots from `keep` on.  into == cache: in place.  Otherwise `into` (same batch, heads and
- * dim; limit >= keep) receives the rows that are kept and `cache` is left as it was.  0 <= recent <= keep. */
+ * dim; limit >= keep) receives the rows that are kept and `cache` is left as it was.  0 <= recent <= keep.  `span` as above. */
 size_t mi_cache_evict_workspace_bytes(const mi_cache_t *cache, int64_t keep);
-int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent,
+int mi_cache_evict(const mi_cache_t *cache, const mi_cache_t *into, int64_t keep, int64_t recent, int64_t span,
                    void *workspace, size_t workspace_bytes, mi_stream_t stream);
 
 #ifdef __cplusplus

@@ -137,7 +137,7 @@ def test_abi_refuses_bad_calls_before_touching_the_device():
     assert L.mi_cache_evict_workspace_bytes(cache(), 10) >= 4 * 10 * 8 and L.mi_cache_evict_workspace_bytes(cache(), 0) == 0
 
     def evict(into=None, keep=10, recent=0, ws=at, nbytes=1 << 30):
-        return L.mi_cache_evict(cache(), into, keep, recent, ws, nbytes, None)
+        return L.mi_cache_evict(cache(), into, keep, recent, 60, ws, nbytes, None)
 
     assert evict(keep=0) == -1 and evict(keep=61) == -1 and evict(recent=-1) == -1 and evict(recent=11) == -1 and evict(ws=None) == -1 and evict(nbytes=8) == -3
     assert evict(into=cache()) == -1 and b"share" in L.mi_last_error()
@@ -422,7 +422,7 @@ def _set_weights(bank, ref, rs, style):
 
 @gpu
 @pytest.mark.parametrize("style", ["spread", "ties", "equal", "special"])
-@pytest.mark.parametrize("dim,fill,keep,recent", [(64, 1, 1, 0), (64, 70, 1, 1), (128, 300, 299, 10), (128, 300, 64, 64), (256, 1000, 37, 5), (72, 5000, 4500, 300), (64, 2500, 1200, 0), (32, 9000, 8500, 100)])
+@pytest.mark.parametrize("dim,fill,keep,recent", [(64, 1, 1, 0), (64, 70, 1, 1), (128, 300, 299, 10), (128, 300, 64, 64), (256, 1000, 37, 5), (72, 5000, 4500, 300), (64, 2500, 1200, 0), (32, 9000, 8500, 100), (64, 20000, 10000, 7), (8, 40000, 15000, 70)])
 def test_evict_in_place_and_into(style, dim, fill, keep, recent):
     rs = np.random.RandomState(fill + keep)
     B, H = 3, 2
