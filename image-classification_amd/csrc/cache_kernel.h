@@ -32,6 +32,7 @@ namespace mi {
 typedef __attribute__((ext_vector_type(8))) __bf16 cb16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 cb16x2;
 typedef __attribute__((ext_vector_type(4))) float cf32x4;
+typedef __attribute__((ext_vector_type(16))) float cf32x16;
 
 enum { CACHE_F32 = 0, CACHE_BF16 = 1, CACHE_F16 = 2 };
 
@@ -95,6 +96,29 @@ __device__ __forceinline__ void store8(void *p, const float (&x)[8])
             }
         }
         *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// N = 2, 4 or 8 of them.
+template <int DT, int N>
+__device__ __forceinline__ void store_n(void *p, const float (&x)[N])
+{
+    if constexpr (N == 8) store8<DT>(p, x);
+    else if constexpr (DT == CACHE_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) ((float2 *)p)[i / 2] = make_float2(x[i], x[i + 1]);
+    } else {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (DT == CACHE_BF16) w[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            else {
+                const _Float16 l = (_Float16)x[2 * i], h = (_Float16)x[2 * i + 1];
+                w[i] = (uint32_t)__builtin_bit_cast(uint16_t, l) | ((uint32_t)__builtin_bit_cast(uint16_t, h) << 16);
+            }
+        }
+        if constexpr (N == 4) *(uint2 *)p = make_uint2(w[0], w[1]);
+        else *(uint32_t *)p = w[0];
     }
 }
 
@@ -259,7 +283,9 @@ struct CacheAttendParams {
     float c2;                                // scale * log2(e)
     float *part;                             // nsplit > 1: [split][batch heads][R][W] partial sums ...
     float2 *part_ml;                         //             ... and [split][batch heads][R] (maximum, sum), maximum in log2 units
-    int chunks;                              // weights: workgroups a (sequence, head), each takes every chunks-th 128 rows
+    int chunks;                              // weights: workgroups along the bank's rows of a (sequence, head); each takes every chunks-th stretch
+    int rsplit;                              // weights, many query rows: pieces of the query rows ...
+    float *part_w;                           //          ... and their sums, [piece][batch heads][rows]
     float *lse;                              // [batch heads][R] log2 of the softmax denominator (weights wanted), or null
     float *scores;                           // [batch heads][R][rows] scores before the scale (few query rows, weights wanted), or null
 };
@@ -325,7 +351,7 @@ __device__ __forceinline__ void load_key(const uint8_t *p, uint32_t (&w)[NB])
     if constexpr (NB == 2) {
         const uint2 v = *(const uint2 *)p;
         w[0] = v.x, w[1] = v.y;
-    } else {
+    } else {                                 // 4, 8 or 16 words
 #pragma unroll
         for (int i = 0; i < NB / 4; ++i) {
             const uint4 v = ((const uint4 *)p)[i];
@@ -605,6 +631,227 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
     }
 }
 
+// Tiled form, for many query rows: a workgroup has 128 of them (32 a wave) and walks over the bank in tiles of 64 rows, which its
+// four waves turn into bf16 once, in shared memory, in the order in which the matrix cores read them (a fragment: 64 lanes x 16
+// bytes).  v_mfma_f32_32x32x16_bf16 (lane = 32 l + c; A: row c, 8 k-values of half l; result: column c, rows 8 (r / 4) + 4 l + r % 4),
+// transposed products as above:
+//   key fragment (token half tt, step i): bank row 32 tt + c, the 8 dims l W/2 + 8 i ...
+//   value fragment (token quarter s, ct): channel c NB + ct, bank rows 16 s + 4 l + {0..3, 8..11}: the rows of which lane (c, l) of
+//   S^T has the probabilities of query row c in registers 8 (s % 2) ...
+template <int NB>
+struct TileRegs {                            // what a wave turns into fragments: NB steps of half of the keys, a quarter of the values
+    uint32_t k[NB], ks[NB == 8 ? 2 : 1], v[8], vs[2];
+};
+
+template <int NB>
+struct TileAt {
+    const uint8_t *k, *ks, *v, *vs;
+    long long scale_ld;
+    __device__ __forceinline__ TileAt(const CacheView &c, long long bh, int lane, int wave)
+    {
+        constexpr int W = 32 * NB;
+        const int l = lane >> 5, cc = lane & 31, half = wave & 1, row = 32 * (wave >> 1) + cc;
+        k = c.key + (bh * c.rows + row) * (W / 2) + l * (W / 4) + half * 4 * NB;
+        ks = c.key_scale + (bh * NB + (l * 2 * NB + half * NB) / 4) * c.rows + row;
+        v = c.value + (bh * c.rows + 16 * wave + 4 * l) * (W / 2) + cc * (NB / 2);
+        vs = c.value_scale + (bh * NB + cc * NB / 32) * c.rows + 16 * wave + 4 * l;
+        scale_ld = c.rows;
+    }
+    __device__ __forceinline__ void load(long long u0, TileRegs<NB> &t) const
+    {
+        load_key<NB>(k + u0 * (16 * NB), t.k);
+        t.ks[0] = ks[u0];
+        if constexpr (NB == 8) t.ks[1] = ks[scale_ld + u0];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint8_t *at = v + (u0 + 8 * (e >> 2) + (e & 3)) * (16 * NB);
+            t.v[e] = NB == 2 ? *at : NB == 4 ? *(const uint16_t *)at : *(const uint32_t *)at;
+        }
+        t.vs[0] = *(const uint32_t *)(vs + u0);
+        t.vs[1] = *(const uint32_t *)(vs + u0 + 8);
+    }
+};
+
+__device__ __forceinline__ uint4 transpose_pairs(const uint32_t (&pair)[8], uint32_t sel)
+{
+    return make_uint4(__builtin_amdgcn_perm(pair[1], pair[0], sel), __builtin_amdgcn_perm(pair[3], pair[2], sel),
+                      __builtin_amdgcn_perm(pair[5], pair[4], sel), __builtin_amdgcn_perm(pair[7], pair[6], sel));
+}
+
+template <int NB>
+__device__ __forceinline__ void store_tile(const TileRegs<NB> &t, uint4 *keys, uint4 *values, int lane, int wave)
+{
+    const int half = wave & 1, tt = wave >> 1;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const uint32_t byte = t.ks[NB == 8 ? i / 4 : 0];
+        uint4 f = __builtin_bit_cast(uint4, cvt8(t.k[i], scale_of(byte)));
+        if (byte == 255) f = make_uint4(0x7fc07fc0u, 0, 0, 0);
+        keys[(tt * 2 * NB + half * NB + i) * 64 + lane] = f;
+    }
+    float sc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[e] = value_scale_of(t.vs[e >> 2], e & 3);
+#pragma unroll
+    for (int i2 = 0; i2 < NB / 2; ++i2) {
+        uint32_t pair[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            pair[e] = i2 == 0 ? cvt2<0>(t.v[e], sc[e]) : i2 == 1 ? cvt2<1>(t.v[e], sc[e]) : i2 == 2 ? cvt2<2>(t.v[e], sc[e]) : cvt2<3>(t.v[e], sc[e]);
+        values[(wave * NB + 2 * i2) * 64 + lane] = transpose_pairs(pair, 0x05040100u);
+        values[(wave * NB + 2 * i2 + 1) * 64 + lane] = transpose_pairs(pair, 0x07060302u);
+    }
+}
+
+// 32 query rows as B operands: lane c = row, half l = dims l W/2 + 8 i.
+template <int DT, int NB, int P>
+__device__ __forceinline__ void load_query32(const CacheAttendParams &p, int b, int h, int row, int l, bool real, int i, cb16x8 (&q)[P])
+{
+    const int t = row / p.G, g = row - t * p.G, d = l * 16 * NB + i * 8;
+    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (real && d < p.c.dim)
+        load8<DT>(p.q + b * p.q_s[0] + (long long)(h * p.G + g) * p.q_s[1] + t * p.q_s[2] + (long long)d * elem_bytes<DT>(), x);
+    split_pieces<P>(x, q);
+}
+
+// Pieces of the probabilities: one for bf16 (2^-8 of each p at most, as much as the result's own rounding may be), as many as the
+// query's for the others.
+template <int DT, int NB>
+__global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_attend_tile_kernel(CacheAttendParams p)
+{
+    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, PP = PQ, KF = 2 * SK, VF = 4 * NB;
+    extern __shared__ uint4 s_tile[];        // [2][KF + VF][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
+    // heads innermost (a head's bank stays in one die's cache where heads are a multiple of 8), the longest rows first
+    const int bhs = p.c.batch * p.c.heads;
+    const long long bh = blockIdx.x % bhs;
+    const int rest = (int)(blockIdx.x / bhs), split = rest % p.nsplit, tile = p.tiles - 1 - rest / p.nsplit;
+    const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
+    int len = p.c.length[b];
+    len = len > p.c.limit ? p.c.limit : len;
+    const int n = real_rows(p.counts, b, p.T);
+
+    const int row = tile * 128 + wave * 32 + c;
+    const bool real = row < p.R && row / p.G < n;
+    const int lim = real ? visible(row / p.G, n, len, p.causal) : 0x7fffffff;      // rows that are not real need no mask: nothing is kept of them
+    int least = lim, most = real ? lim : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        least = min(least, __shfl_xor(least, d));
+        most = max(most, __shfl_xor(most, d));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    // the workgroup's most: its last real row sees as much as any
+    const int t_last = min(min(tile * 128 + 127, p.R - 1) / p.G, n - 1);
+    const int all_most = t_last < tile * 128 / p.G ? 0 : visible(t_last, n, len, p.causal);
+    const int units = (all_most + 63) / 64, per = (units + p.nsplit - 1) / p.nsplit, first = split * per, last = min(units, first + per);
+
+    cb16x8 q[SK][PQ];
+#pragma unroll
+    for (int i = 0; i < SK; ++i) load_query32<DT, NB, PQ>(p, b, h, real ? row : 0, l, real, i, q[i]);
+    cf32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    float mx = -INFINITY, ref = 0.f, sum = 0.f;
+
+    if (first < last) {
+        const TileAt<NB> at(p.c, bh, lane, wave);
+        TileRegs<NB> t;
+        at.load(first * 64, t);
+        store_tile<NB>(t, s_tile, s_tile + KF * 64, lane, wave);
+        at.load(min(first + 1, last - 1) * 64, t);
+        __syncthreads();
+        for (int un = first; un < last; ++un) {
+            const uint4 *keys = s_tile + ((un - first) & 1) * (KF + VF) * 64, *values = keys + KF * 64;
+            const int u0 = un * 64;
+            if (u0 < most) {
+                cf32x16 s[2];
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < SK; ++i)
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) {
+                        const cb16x8 kf = __builtin_bit_cast(cb16x8, keys[(tt * SK + i) * 64 + lane]);
+#pragma unroll
+                        for (int k = 0; k < PQ; ++k) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], s[tt], 0, 0, 0);
+                    }
+                if (u0 + 64 > least) {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r)
+                        if (u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3) >= lim) s[r >> 4][r & 15] = -INFINITY;
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int r = 1; r < 32; ++r) top = fmaxf(top, s[r >> 4][r & 15]);
+                if (__any(top > mx)) {
+                    const float now = fmaxf(mx, fmaxf(top, __shfl_xor(top, 32)));
+                    ref = now == -INFINITY ? 0.f : now * p.c2;
+                    const float shrink = __builtin_amdgcn_exp2f(fmaf(mx, p.c2, -ref));
+                    mx = now;
+                    sum *= shrink;
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) o[i] *= shrink;
+                }
+#pragma unroll
+                for (int sq = 0; sq < 4; ++sq) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(fmaf(s[sq >> 1][(sq & 1) * 8 + e], p.c2, -ref));
+                        sum += x[e];
+                    }
+                    cb16x8 pf[PP];
+                    split_pieces<PP>(x, pf);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        const cb16x8 vf = __builtin_bit_cast(cb16x8, values[(sq * NB + i) * 64 + lane]);
+#pragma unroll
+                        for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[i], 0, 0, 0);
+                    }
+                }
+            }
+            if (un + 1 < last) {
+                uint4 *to = s_tile + ((un + 1 - first) & 1) * (KF + VF) * 64;
+                store_tile<NB>(t, to, to + KF * 64, lane, wave);
+                at.load(min(un + 2, last - 1) * 64, t);
+            }
+            __syncthreads();
+        }
+    }
+    sum += __shfl_xor(sum, 32);
+    if (row >= p.R) return;
+    const bool none = !real || mx == -INFINITY;
+    const int tq = row / p.G, g = row - tq * p.G;
+    if (p.nsplit > 1) {
+        const long long gr = ((long long)split * bhs + bh) * p.R + row;
+        float *to = p.part + gr * W;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) to[(8 * (r >> 2) + 4 * l + (r & 3)) * NB + i] = o[i][r];
+        if (l == 0) p.part_ml[gr] = make_float2(none ? -INFINITY : ref, sum);
+        return;
+    }
+    const float inv = 1.f / sum;
+    char *to = p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + tq * p.out_s[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int d = (8 * (r >> 2) + 4 * l + (r & 3)) * NB;
+        if (d >= p.c.dim) continue;
+        float x[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) x[i] = none ? 0.f : o[i][r] * inv;
+        store_n<DT, NB>(to + (long long)d * elem_bytes<DT>(), x);
+    }
+    if (p.lse && l == 0) p.lse[bh * p.R + row] = none ? INFINITY : ref + __builtin_amdgcn_logf(sum);
+}
+
 // Joins the pieces of a row, one workgroup a row: W / 8 lanes side by side in a piece, 2048 / W pieces at a time.  (One lane
 // group a row, walking over the pieces, took 152 us for 256 pieces of 32 rows: a chain of dependent loads.)
 constexpr int CACHE_MAX_SPLIT = 256;
@@ -712,6 +959,137 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
             const int slot = u0 + 16 * (e >> 2) + 4 * j + (e & 3);
             if (c == e && slot < len) p.c.weight[bh * p.c.rows + slot] += w[e];
         }
+    }
+}
+
+// The same for many query rows: a wave keeps 64 bank rows as operands and the workgroup's four waves share tiles of 32 query rows
+// through shared memory.  Where bank rows are few, the query rows are cut into `rsplit` pieces, whose sums are added up after.
+template <int DT, int NB>
+__global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_weigh_tile_kernel(CacheAttendParams p)
+{
+    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, MINE = SK / 4;      // steps of a query tile that a wave loads: NB / 2
+    static_assert(MINE * 4 == SK, "four waves");
+    __shared__ uint4 s_q[2][SK * PQ][64];
+    __shared__ float s_lse[2][32];
+    __shared__ int s_lim[2][32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
+    const int bhs = p.c.batch * p.c.heads;
+    const long long bh = blockIdx.x % bhs;
+    const int rest = (int)(blockIdx.x / bhs), piece = rest % p.rsplit, chunk = rest / p.rsplit;
+    const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
+    int len = p.c.length[b];
+    len = len > p.c.limit ? p.c.limit : len;
+    const int n = real_rows(p.counts, b, p.T);
+    const int tiles = (int)(((long long)n * p.G + 31) / 32), per = (tiles + p.rsplit - 1) / p.rsplit;
+    for (int w0 = chunk * 256; w0 < len; w0 += p.chunks * 256) {
+        const int u0 = w0 + wave * 64;
+        cb16x8 kf[2][SK];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const long long at = min(u0 + 32 * tt + c, p.c.rows - 1);                // rows past the allocation: any row, left out below
+            const uint8_t *k = p.c.key + (bh * p.c.rows + at) * (W / 2) + l * (W / 4);
+            uint32_t w[SK];
+            load_key<SK>(k, w);
+#pragma unroll
+            for (int i = 0; i < SK; ++i) {
+                const uint32_t byte = p.c.key_scale[(bh * NB + (l * SK + i) / 4) * p.c.rows + at];
+                uint4 f = __builtin_bit_cast(uint4, cvt8(w[i], scale_of(byte)));
+                if (byte == 255) f = make_uint4(0x7fc07fc0u, 0, 0, 0);
+                kf[tt][i] = __builtin_bit_cast(cb16x8, f);
+            }
+        }
+        float w[32];
+#pragma unroll
+        for (int r = 0; r < 32; ++r) w[r] = 0.f;
+        // tiles before the first row that sees slot w0 are left out
+        const long long row_lo = (p.causal ? max(0, w0 - (len - n)) : 0) * (long long)p.G;
+        const int first = max(piece * per, (int)min((long long)tiles, row_lo / 32)), last = min(tiles, (piece + 1) * per);
+        uint4 mine[MINE * PQ];
+        float lse = 0.f;
+        int lim = 0;
+        const auto fetch = [&](int tile) {
+            const int row = tile * 32 + c;
+            const bool in = row < p.R && row / p.G < n;
+            lim = in ? visible(row / p.G, n, len, p.causal) : 0;
+            lse = lim > 0 ? p.lse[bh * p.R + row] : INFINITY;
+#pragma unroll
+            for (int m = 0; m < MINE; ++m) {
+                cb16x8 q[PQ];
+                load_query32<DT, NB, PQ>(p, b, h, in ? row : 0, l, lim > 0, wave * MINE + m, q);
+#pragma unroll
+                for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
+            }
+        };
+        const auto leave = [&](int buf) {
+#pragma unroll
+            for (int m = 0; m < MINE * PQ; ++m) s_q[buf][wave * MINE * PQ + m][lane] = mine[m];
+            if (wave == 0 && l == 0) s_lse[buf][c] = lse, s_lim[buf][c] = lim;
+        };
+        __syncthreads();
+        if (first < last) {
+            fetch(first);
+            leave(0);
+            fetch(min(first + 1, last - 1));
+        }
+        __syncthreads();
+        for (int tile = first; tile < last; ++tile) {
+            const int buf = (tile - first) & 1;
+            cf32x16 s[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < SK; ++i)
+#pragma unroll
+                for (int k = 0; k < PQ; ++k) {
+                    const cb16x8 q = __builtin_bit_cast(cb16x8, s_q[buf][i * PQ + k][lane]);
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[tt][i], q, s[tt], 0, 0, 0);
+                }
+            const float off = s_lse[buf][c];
+            const int sees = s_lim[buf][c];
+            if (__all(sees >= u0 + 64)) {
+#pragma unroll
+                for (int r = 0; r < 32; ++r) w[r] += __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], p.c2, -off));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], p.c2, -off));
+                    w[r] += u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3) < sees ? x : 0.f;
+                }
+            }
+            if (tile + 1 < last) {
+                leave(buf ^ 1);
+                fetch(min(tile + 2, last - 1));
+            }
+            __syncthreads();
+        }
+        float *to = p.rsplit > 1 ? p.part_w + ((long long)piece * bhs + bh) * p.c.rows : p.c.weight + bh * p.c.rows;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) w[r] += __shfl_xor(w[r], d);
+            const int slot = u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3);
+            if (c == r && slot < len) {
+                if (p.rsplit > 1) to[slot] = w[r];
+                else to[slot] += w[r];
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void cache_weigh_add_kernel(CacheAttendParams p)
+{
+    const int bhs = p.c.batch * p.c.heads;
+    const long long bh = blockIdx.x % bhs;
+    int len = p.c.length[bh / p.c.heads];
+    len = len > p.c.limit ? p.c.limit : len;
+    const int step = (int)(gridDim.x / bhs) * 256;
+    for (int slot = (int)(blockIdx.x / bhs) * 256 + threadIdx.x; slot < len; slot += step) {
+        float w = p.c.weight[bh * p.c.rows + slot];
+        for (int s = 0; s < p.rsplit; ++s) w += p.part_w[((long long)s * bhs + bh) * p.c.rows + slot];
+        p.c.weight[bh * p.c.rows + slot] = w;
     }
 }
 

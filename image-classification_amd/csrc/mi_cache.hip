@@ -71,9 +71,10 @@ int check_grid(const char *who, int64_t blocks)
 // there are few of them.
 struct AttendPlan {
     int64_t R, mt, tiles, nsplit;
-    int64_t chunks;                          // weights: workgroups a (sequence, head)
+    bool tiled;                              // 128 query rows a workgroup through shared memory, not 16 mt straight from memory
+    int64_t chunks, rsplit;                  // weights: workgroups a (sequence, head) along the bank, and along the query rows
     bool scores;                             // weights: from scores left behind, not from a second product
-    size_t off_ml, off_lse, off_scores, total;
+    size_t off_ml, off_lse, off_scores, off_w, total;
 };
 
 AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
@@ -83,10 +84,11 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     a.mt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
     const int64_t wide = (width_of(c->dim) == 256 ? 2 : 4) / (dtype == MI_F32 ? 2 : 1);      // what the register file holds
     if (a.mt > wide) a.mt = wide;
-    a.tiles = ceil_div(a.R, 16 * a.mt);
-    const int64_t groups = c->batch * c->heads * a.tiles;
+    a.tiled = a.R >= 64;
+    a.tiles = ceil_div(a.R, a.tiled ? 128 : 16 * a.mt);
+    const int64_t bh = c->batch * c->heads, groups = bh * a.tiles;
     span = span < 1 ? 1 : span > c->limit ? c->limit : span;
-    int64_t ns = ceil_div(768, groups);
+    int64_t ns = ceil_div(a.tiled ? 512 : 768, groups);
     const int64_t most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
     a.nsplit = ns < 1 ? 1 : ns > most ? most : ns;
     const int64_t rows = c->batch * c->heads * a.R;
@@ -102,7 +104,14 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     // product once more.  Scores are laid out by the capacity (a captured call may see longer sequences than `span`).
     const int64_t score_bytes = rows * c->rows * 4;
     a.scores = accumulate && a.mt == 1 && 8 * a.R <= width_of(c->dim) / 2 && score_bytes <= ((int64_t)1 << 30);
-    a.chunks = ceil_div(span, a.scores ? 1024 : 128);
+    a.chunks = ceil_div(span, a.scores ? 1024 : a.tiled ? 256 : 128);
+    a.rsplit = 1;
+    if (accumulate && a.tiled) {
+        a.rsplit = std::min<int64_t>(std::max<int64_t>(1, 512 / (bh * a.chunks)), ceil_div(a.R, 256));
+        while (a.rsplit > 1 && a.rsplit * bh * c->rows * 4 > ((int64_t)1 << 30)) --a.rsplit;
+        a.off_w = at;
+        if (a.rsplit > 1) at += (size_t)(a.rsplit * bh * c->rows * 4);
+    }
     a.off_scores = at;
     if (a.scores) at += (size_t)score_bytes;
     a.total = at < 256 ? 256 : at;
@@ -114,15 +123,24 @@ hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, in
 {
     const int64_t bh = (int64_t)p.c.batch * p.c.heads;
     const dim3 grid((unsigned)(bh * a.tiles * a.nsplit));
-    if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
+    if (a.tiled) {
+        const size_t lds = (size_t)NB * 16 * 1024;         // two tiles of 64 rows, keys and values in bf16
+        static std::atomic<uint64_t> done{0};
+        const hipError_t e = ensure_dynamic_lds(mi::cache_attend_tile_kernel<DT, NB>, lds, done);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((mi::cache_attend_tile_kernel<DT, NB>), grid, dim3(256), lds, s, p);
+    } else if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
     if constexpr (NB < 8 || DT != mi::CACHE_F32)
-        if (a.mt == 2) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 2>), grid, dim3(256), 0, s, p);
+        if (!a.tiled && a.mt == 2) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 2>), grid, dim3(256), 0, s, p);
     if constexpr (NB < 8 && DT != mi::CACHE_F32)
-        if (a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
+        if (!a.tiled && a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
     if (a.nsplit > 1)
         hipLaunchKernelGGL((mi::cache_join_kernel<DT, 32 * NB>), dim3((unsigned)(bh * a.R)), dim3(256), 0, s, p);
     if (a.scores) hipLaunchKernelGGL(mi::cache_weigh_scores_kernel, dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
-    else if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
+    else if (accumulate && a.tiled) {
+        hipLaunchKernelGGL((mi::cache_weigh_tile_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks * a.rsplit)), dim3(256), 0, s, p);
+        if (a.rsplit > 1) hipLaunchKernelGGL(mi::cache_weigh_add_kernel, dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
+    } else if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -230,7 +248,7 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     const int64_t bh = cache->batch * cache->heads;
     MI_TRY(check_grid("mi_cache_attend", bh * a.tiles * a.nsplit));
     MI_TRY(check_grid("mi_cache_attend", bh * a.R));
-    MI_TRY(check_grid("mi_cache_attend", bh * a.chunks));
+    MI_TRY(check_grid("mi_cache_attend", bh * a.chunks * a.rsplit));
     p.c = view(cache);
     p.q = (const char *)query;
     p.out = (char *)out;
@@ -240,6 +258,8 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     p.c2 = scale * mi::CACHE_LOG2E;
     p.part = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + a.off_ml);
+    p.rsplit = (int)a.rsplit;
+    p.part_w = (float *)((char *)workspace + a.off_w);
     p.scores = a.scores ? (float *)((char *)workspace + a.off_scores) : nullptr;
     p.lse = accumulate ? (float *)((char *)workspace + a.off_lse) : nullptr;
     hipStream_t s = (hipStream_t)stream;

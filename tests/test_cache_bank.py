@@ -1,8 +1,9 @@
 """CacheBank: keys and values in 4 bits, attention over them, eviction.  Kernels against tests/cache_ref.py (numpy, 64 bits).
 
 What is held is compared bit for bit (values on a grid times a power of two), eviction too.  Attention outputs are off by half a step of
-their type (finfo.eps / 2) and the float32 bound that cache_ref.RefBank.attend derives; bfloat16 and float16 results carry probabilities
-in two bf16 pieces (2^-17 of each, relative), float32 ones in three."""
+their type (finfo.eps / 2) and the float32 bound that cache_ref.RefBank.attend derives.  Probabilities enter the second product in bf16
+pieces: three for float32 queries (2^-24 of each p is left out), two for float16 and for few rows of bfloat16 (2^-17), one for 64 or more
+bfloat16 rows of a head: that rounds each p by at most 2^-8 of itself, so the result by at most 2^-8 sum p|v|."""
 import copy
 
 import numpy as np
@@ -54,9 +55,9 @@ def _rows_equal(bank, ref, name="kv"):
         assert not keys[b, :, n:].any() and not values[b, :, n:].any()
 
 
-def _check_out(out, want, bound, dtype):
+def _check_out(out, want, bound, dtype, rows=1):
     got = _np(out)
-    tail = 2.0 ** -17 if dtype != "fp32" else 2.0 ** -24
+    tail = 2.0 ** -24 if dtype == "fp32" else 2.0 ** -8 if dtype == "bf16" and rows >= 64 else 2.0 ** -17
     assert np.array_equal(np.isnan(got), np.isnan(want))
     ok = ~np.isnan(want)
     info = torch.finfo(DT[dtype])
@@ -279,7 +280,7 @@ def test_attend_against_64_bits(dtype, dim, H, group, T, fill):
             out = bank.attend("kv", q.cuda(), counts=counts, causal=causal, accumulate=accumulate)
             want = ref.attend(_np(q), counts, causal=causal, accumulate=accumulate)
             assert out.dtype == DT[dtype] and out.shape == q.shape
-            _check_out(out, want[0], want[1], dtype)
+            _check_out(out, want[0], want[1], dtype, T * group)
             if accumulate:
                 for b in range(B):
                     for h in range(H):
@@ -482,7 +483,7 @@ def test_generation_under_a_budget(dtype):
         ref.push(_np(kv[0]), _np(kv[1]), counts)
         out = bank.attend("kv", q.cuda(), counts=counts, accumulate=True)
         want, bound, wb = ref.attend(_np(q), counts, accumulate=True)
-        _check_out(out, want, bound, dtype)
+        _check_out(out, want, bound, dtype, T * group)
         for b in range(B):
             for h in range(H):
                 got = _np(bank.weights("kv"))[b, h, :ref.length(b)]
