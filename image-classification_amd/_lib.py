@@ -97,7 +97,7 @@ def lib() -> ctypes.CDLL:
     L.mi_cache_trim.restype, L.mi_cache_trim.argtypes = i32, [cache, p, i64, p]
     L.mi_cache_read.restype, L.mi_cache_read.argtypes = i32, [cache, p, p, p]
     L.mi_cache_attend_workspace_bytes.restype = sz
-    L.mi_cache_attend_workspace_bytes.argtypes = [cache, i32, i64, i64, i64, i32]
+    L.mi_cache_attend_workspace_bytes.argtypes = [cache, i32, i64, i64, i64, i32, i32]
     L.mi_cache_attend.restype = i32
     L.mi_cache_attend.argtypes = [cache, p, strides, p, strides, i32, i64, i64, p, f32, i32, i32, i64, p, sz, p]
     L.mi_cache_evict_workspace_bytes.restype = sz

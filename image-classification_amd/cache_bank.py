@@ -211,7 +211,7 @@ class CacheBank(nn.Module):
                 return out
             span = max(1, self.sizes[name] if name in self._captured else self._bounds[name])
             code = _CODES[query.dtype]
-            nbytes = L.mi_cache_attend_workspace_bytes(ctypes.byref(view), code, T, group, span, int(accumulate))
+            nbytes = L.mi_cache_attend_workspace_bytes(ctypes.byref(view), code, T, group, span, int(causal), int(accumulate))
             ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
             _lib.check(L.mi_cache_attend(ctypes.byref(view), query.data_ptr(), (ctypes.c_int64 * 3)(*_strides(query)),
                                          out.data_ptr(), (ctypes.c_int64 * 3)(*_strides(out)), code, T, group,

@@ -6,7 +6,8 @@
 // to [-126, 125] and stored as the byte e + 127.  Elements are x / 2^e on E2M1 (0 .5 1 1.5 2 3 4 6, sign bit), nearest even,
 // saturating; two a byte, the even one in the low four bits.  Every element times its scale is exact in bf16, which is what
 // the matrix cores read: v_cvt_scalef32_pk_bf16_fp4 turns two elements and their scale into two bf16 in one instruction.
-// A row (of one head) whose key or value has a NaN or an infinity is held as NaN whole: scale bytes 255, elements 0.
+// A row (of one head) whose key or value has a NaN or an infinity is held as NaN whole: scale bytes 255 on its key (0 on its
+// value, so that a product with a probability of zero stays zero), elements 0.
 //
 //   key, value              [batch][heads][rows][W / 2]   bytes
 //   key_scale, value_scale  [batch][heads][W / 32][rows]  bytes: rows innermost, so that a lane of the value product gets the
@@ -26,6 +27,8 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 namespace mi {
 
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
         const long long slot = (long long)len + t;
         *(uint32_t *)((side ? p.c.value : p.c.key) + (bh * p.c.rows + slot) * (W / 2) + c * 4) = code;
         if ((c & 3) == 0)
-            (side ? p.c.value_scale : p.c.key_scale)[(bh * (W / 32) + c / 4) * p.c.rows + slot] = (uint8_t)(poison ? 255 : byte);
+            (side ? p.c.value_scale : p.c.key_scale)[(bh * (W / 32) + c / 4) * p.c.rows + slot] = (uint8_t)(!poison ? byte : side ? 0 : 255);
         if (c == 0) {
             if (side) p.c.position[bh * p.c.rows + slot] = p.c.seen[b] + t;
             else p.c.weight[bh * p.c.rows + slot] = 0.f;
@@ -264,7 +267,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, uint4 *key
         v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1));
         v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2));
         v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3));
-        if (byte == 255) v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        const bool nan = (side ? c.key_scale[(bh * (W / 32) + d / 4) * c.rows + slot] : byte) == 255;
+        if (nan) v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
     }
     (side ? value : key)[r * (c.dim / 8) + d] = v;
 }
@@ -306,7 +310,8 @@ __device__ __forceinline__ int real_rows(const int *counts, int b, int T)
 
 // 8 values as 1..3 bf16 pieces whose sum is the value: 8 bits of significand each (bf16: exact with one, float16: with two,
 // float32: with three).  A piece of an infinity or NaN is that value itself, the rest zero.
-template <int P>
+// Probabilities need no such care: what is left of a NaN is a NaN.
+template <int P, bool CARE = true>
 __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[P])
 {
 #pragma unroll
@@ -317,7 +322,7 @@ __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[
             const __bf16 h = (__bf16)v;
             out[k][i] = h;
             v = v - (float)h;
-            if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.f;
+            if (CARE && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.f;
         }
     }
 }
@@ -325,12 +330,7 @@ __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[
 template <int DT> struct Pieces { static constexpr int N = DT == CACHE_F32 ? 3 : DT == CACHE_F16 ? 2 : 1; };
 
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-// a value's scale is kept finite: a NaN row has reached the result through its key, and 0 * inf must not reach other rows
-__device__ __forceinline__ float value_scale_of(uint32_t word, int e)
-{
-    const uint32_t bits = e == 3 ? (word >> 1) & 0x7f800000u : (word << (23 - 8 * e)) & 0x7f800000u;
-    return __uint_as_float(bits < 0x7f000000u ? bits : 0x7f000000u);
-}
+__device__ __forceinline__ float scale_of(uint32_t word, int e) { return __uint_as_float(((word >> (8 * e)) & 255u) << 23); }
 
 template <int I>
 __device__ __forceinline__ uint32_t cvt2(uint32_t w, float s)
@@ -421,9 +421,9 @@ __device__ __forceinline__ cb16x8 key_operand(const uint32_t (&k)[NB], const uin
 {
     const uint32_t byte = ks[NB == 8 ? i / 4 : 0];
     cb16x8 f = cvt8(k[i], scale_of(byte));
-    if (i % 4 == 0 && byte == 255) {
+    if (i == 0) {
         uint4 v = __builtin_bit_cast(uint4, f);
-        v = make_uint4(0x7fc07fc0u, 0, 0, 0);
+        v.x = byte == 255 ? 0x7fc07fc0u : v.x;
         f = __builtin_bit_cast(cb16x8, v);
     }
     return f;
@@ -458,7 +458,7 @@ __device__ __forceinline__ float across_j_sum(float x)
 // Streaming form: a workgroup has MT tiles of 16 query rows of one (sequence, head) and one piece of its bank rows; its four
 // waves take every fourth unit of 32 rows each, straight from memory into registers, and are joined at the end.
 template <int DT, int NB, int MT>
-__global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
+__global__ __launch_bounds__(256, MT == 1 && NB < 8 ? 2 : 1) void cache_attend_kernel(CacheAttendParams p)
 {
     constexpr int W = 32 * NB, PQ = Pieces<DT>::N, PP = DT == CACHE_F32 ? 3 : 2, LD = W + 4;
     __shared__ float s_m[4][16], s_l[4][16];
@@ -558,14 +558,14 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
                 x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], p.c2, -ref[m]));
                 sum[m] += x[e];
             }
-            split_pieces<PP>(x, pf[m]);
+            split_pieces<PP, false>(x, pf[m]);
         }
 #pragma unroll
         for (int i2 = 0; i2 < NB; ++i2) {                 // channels 2 i2, 2 i2 + 1 of each lane
             uint32_t pair[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float sc = value_scale_of(u.vs[e >> 2], e & 3);
+                const float sc = scale_of(u.vs[e >> 2], e & 3);
                 const uint32_t w = u.v[e][NB == 8 ? i2 / 4 : 0];
                 pair[e] = i2 % 4 == 0 ? cvt2<0>(w, sc) : i2 % 4 == 1 ? cvt2<1>(w, sc) : i2 % 4 == 2 ? cvt2<2>(w, sc) : cvt2<3>(w, sc);
             }
@@ -619,27 +619,27 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(CacheAttendParams p)
             if (p.nsplit > 1) {
                 const long long g = ((long long)split * p.c.batch * p.c.heads + bh) * p.R + row;
                 store8<CACHE_F32>(p.part + g * W + d, x);
-                if (d == 0) p.part_ml[g] = make_float2(big == -INFINITY ? -INFINITY : rref, den);
+                if (d == 0) p.part_ml[g] = make_float2(den == 0.f ? -INFINITY : rref, den);
             } else {
-                const float inv = big == -INFINITY ? 0.f : 1.f / den;
-                for (int i = 0; i < 8; ++i) x[i] = big == -INFINITY ? 0.f : x[i] * inv;
+                const float inv = 1.f / den;                      // (a row that sees nothing but NaN is NaN, one that sees nothing is zero)
+                for (int i = 0; i < 8; ++i) x[i] = den == 0.f ? 0.f : x[i] * inv;
                 const int t = row / p.G, g = row - t * p.G;
                 if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-                if (p.lse && d == 0) p.lse[bh * p.R + row] = big == -INFINITY ? INFINITY : rref + __builtin_amdgcn_logf(den);
+                if (p.lse && d == 0) p.lse[bh * p.R + row] = den == 0.f ? INFINITY : rref + __builtin_amdgcn_logf(den);
             }
         }
     }
 }
 
-// Tiled form, for many query rows: a workgroup has 128 of them (32 a wave) and walks over the bank in tiles of 64 rows, which its
-// four waves turn into bf16 once, in shared memory, in the order in which the matrix cores read them (a fragment: 64 lanes x 16
-// bytes).  v_mfma_f32_32x32x16_bf16 (lane = 32 l + c; A: row c, 8 k-values of half l; result: column c, rows 8 (r / 4) + 4 l + r % 4),
-// transposed products as above:
-//   key fragment (token half tt, step i): bank row 32 tt + c, the 8 dims l W/2 + 8 i ...
-//   value fragment (token quarter s, ct): channel c NB + ct, bank rows 16 s + 4 l + {0..3, 8..11}: the rows of which lane (c, l) of
+// Tiled form, for many query rows: each of a workgroup's WAVES waves has 32 of them, and the workgroup walks over the bank in tiles
+// of 16 WAVES rows, which its waves turn into bf16 once, in shared memory, in the order in which the matrix cores read them (a
+// fragment: 64 lanes x 16 bytes).  v_mfma_f32_32x32x16_bf16 (lane = 32 l + c; A: row c, 8 k-values of half l; result: column c,
+// rows 8 (r / 4) + 4 l + r % 4), transposed products as above:
+//   key fragment (32 bank rows tt, step i): bank row 32 tt + c, the 8 dims l W/2 + 8 i ...
+//   value fragment (16 bank rows s, ct): channel c NB + ct, bank rows 16 s + 4 l + {0..3, 8..11}: the rows of which lane (c, l) of
 //   S^T has the probabilities of query row c in registers 8 (s % 2) ...
 template <int NB>
-struct TileRegs {                            // what a wave turns into fragments: NB steps of half of the keys, a quarter of the values
+struct TileRegs {                            // what a wave turns into fragments: NB of the 2 NB steps of 32 keys, 16 values
     uint32_t k[NB], ks[NB == 8 ? 2 : 1], v[8], vs[2];
 };
 
@@ -686,12 +686,12 @@ __device__ __forceinline__ void store_tile(const TileRegs<NB> &t, uint4 *keys, u
     for (int i = 0; i < NB; ++i) {
         const uint32_t byte = t.ks[NB == 8 ? i / 4 : 0];
         uint4 f = __builtin_bit_cast(uint4, cvt8(t.k[i], scale_of(byte)));
-        if (byte == 255) f = make_uint4(0x7fc07fc0u, 0, 0, 0);
+        if (i == 0) f.x = byte == 255 ? 0x7fc07fc0u : f.x;
         keys[(tt * 2 * NB + half * NB + i) * 64 + lane] = f;
     }
     float sc[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sc[e] = value_scale_of(t.vs[e >> 2], e & 3);
+    for (int e = 0; e < 8; ++e) sc[e] = scale_of(t.vs[e >> 2], e & 3);
 #pragma unroll
     for (int i2 = 0; i2 < NB / 2; ++i2) {
         uint32_t pair[8];
@@ -714,12 +714,25 @@ __device__ __forceinline__ void load_query32(const CacheAttendParams &p, int b, 
     split_pieces<P>(x, q);
 }
 
-// Pieces of the probabilities: one for bf16 (2^-8 of each p at most, as much as the result's own rounding may be), as many as the
-// query's for the others.
-template <int DT, int NB>
-__global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_attend_tile_kernel(CacheAttendParams p)
+// x + the sum of the two halves of a word of bf16, in float32 and one instruction.
+__device__ __forceinline__ float add_pair(uint32_t pair, float x)
 {
-    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, PP = PQ, KF = 2 * SK, VF = 4 * NB;
+    const uint32_t ones = 0x3f803f80u;
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(cb16x2, pair), __builtin_bit_cast(cb16x2, ones), x, false);
+}
+
+// How much a score may pass the reference of the exponent (in powers of two) before sums are rescaled: float32 and bf16 have the
+// range, and with it the reference hardly ever moves after the first tile.
+constexpr float CACHE_SLACK = 16.f;
+
+// Pieces of the probabilities: one for bf16 (2^-8 of each p at most, as much as the result's own rounding may be), as many as the
+// query's for the others.  The denominator sums the rounded p of bf16, a pair an instruction; where attention sums divide by it too
+// (EXACT) and for the other types it sums p as it is (prompt of 4096, 32 heads on 8: 164 us with pairs, 194 us without).
+template <int DT, int NB, int WAVES, bool EXACT>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_attend_tile_kernel(CacheAttendParams p)
+{
+    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, PP = PQ, ROWS = 32 * WAVES, TOKENS = 16 * WAVES, SUB = TOKENS / 32;
+    constexpr int KF = SUB * SK, VF = WAVES * NB;                 // fragments of a tile
     extern __shared__ uint4 s_tile[];        // [2][KF + VF][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
     // heads innermost (a head's bank stays in one die's cache where heads are a multiple of 8), the longest rows first
@@ -731,111 +744,143 @@ __global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache
     len = len > p.c.limit ? p.c.limit : len;
     const int n = real_rows(p.counts, b, p.T);
 
-    const int row = tile * 128 + wave * 32 + c;
+    const int row = tile * ROWS + wave * 32 + c;
     const bool real = row < p.R && row / p.G < n;
     const int lim = real ? visible(row / p.G, n, len, p.causal) : 0x7fffffff;      // rows that are not real need no mask: nothing is kept of them
-    int least = lim, most = real ? lim : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        least = min(least, __shfl_xor(least, d));
-        most = max(most, __shfl_xor(most, d));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-    // the workgroup's most: its last real row sees as much as any
-    const int t_last = min(min(tile * 128 + 127, p.R - 1) / p.G, n - 1);
-    const int all_most = t_last < tile * 128 / p.G ? 0 : visible(t_last, n, len, p.causal);
-    const int units = (all_most + 63) / 64, per = (units + p.nsplit - 1) / p.nsplit, first = split * per, last = min(units, first + per);
+    // the workgroup's first row sees least of its real ones, the last one most
+    const int t_first = tile * ROWS / p.G, t_last = min(min(tile * ROWS + ROWS - 1, p.R - 1) / p.G, n - 1);
+    const int least = t_last < t_first ? 0 : visible(t_first, n, len, p.causal), most = t_last < t_first ? 0 : visible(t_last, n, len, p.causal);
+    // pieces are as long for every tile (causal: the first tiles have fewer of them)
+    const int units = (most + TOKENS - 1) / TOKENS, per = ((len + TOKENS - 1) / TOKENS + p.nsplit - 1) / p.nsplit, first = split * per, last = min(units, first + per);
 
     cb16x8 q[SK][PQ];
 #pragma unroll
     for (int i = 0; i < SK; ++i) load_query32<DT, NB, PQ>(p, b, h, real ? row : 0, l, real, i, q[i]);
-    cf32x16 o[NB];
+    cf32x16 o[NB], s[SUB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-    float mx = -INFINITY, ref = 0.f, sum = 0.f;
+    float ref = -INFINITY, sum = 0.f, top = -INFINITY;            // reference of the exponent (log2 units), sum, largest score of a tile
 
     if (first < last) {
-        const TileAt<NB> at(p.c, bh, lane, wave);
+        const TileAt<NB> at(p.c, bh, lane, wave & 3);
         TileRegs<NB> t;
-        at.load(first * 64, t);
-        store_tile<NB>(t, s_tile, s_tile + KF * 64, lane, wave);
-        at.load(min(first + 1, last - 1) * 64, t);
+        // four waves have 64 rows of a tile; where those lie past the allocation (a multiple of 64), its last 64 stand in: they are masked
+        const auto load = [&](int un) { at.load(min(min(un, last - 1) * TOKENS + 64 * (wave >> 2), p.c.rows - 64), t); };
+        const auto leave = [&](int un) {
+            uint4 *to = s_tile + ((un - first) & 1) * (KF + VF) * 64;
+            store_tile<NB>(t, to, to + KF * 64, lane, wave);
+        };
+        // scores of a tile and the largest of them
+        const auto product = [&](int un, auto masked) {
+            const uint4 *keys = s_tile + ((un - first) & 1) * (KF + VF) * 64;
+#pragma unroll
+            for (int tt = 0; tt < SUB; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < SK; ++i)
+#pragma unroll
+                for (int tt = 0; tt < SUB; ++tt) {
+                    const cb16x8 kf = __builtin_bit_cast(cb16x8, keys[(tt * SK + i) * 64 + lane]);
+#pragma unroll
+                    for (int k = 0; k < PQ; ++k) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], s[tt], 0, 0, 0);
+                }
+            if constexpr (decltype(masked)::value) {
+                const int left = lim - un * TOKENS - 4 * l;
+#pragma unroll
+                for (int r = 0; r < 16 * SUB; ++r)
+                    if (32 * (r >> 4) + 8 * ((r & 15) >> 2) + (r & 3) >= left) s[r >> 4][r & 15] = -INFINITY;
+            }
+            top = s[0][0];
+#pragma unroll
+            for (int r = 1; r < 16 * SUB; ++r) top = fmaxf(top, s[r >> 4][r & 15]);
+        };
+        const auto moved = [&]() { return __any(fmaf(top, p.c2, -CACHE_SLACK) > ref); };
+        const auto rescale = [&]() {
+            const float now = fmaxf(ref, fmaxf(top, __shfl_xor(top, 32)) * p.c2);
+            const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
+            ref = now;
+            sum *= shrink;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) o[i] *= shrink;
+        };
+        const auto apply = [&](int un) {
+            const uint4 *values = s_tile + ((un - first) & 1) * (KF + VF) * 64 + KF * 64;
+            const float off = ref == -INFINITY ? 0.f : -ref;
+#pragma unroll
+            for (int sq = 0; sq < 2 * SUB; ++sq) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[sq >> 1][(sq & 1) * 8 + e], p.c2, off));
+                    if constexpr (EXACT) sum += x[e];
+                }
+                cb16x8 pf[PP];
+                split_pieces<PP, false>(x, pf);
+                if constexpr (!EXACT) {
+                    const uint4 w = __builtin_bit_cast(uint4, pf[0]);
+                    sum = add_pair(w.x, add_pair(w.y, add_pair(w.z, add_pair(w.w, sum))));
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const cb16x8 vf = __builtin_bit_cast(cb16x8, values[(sq * NB + i) * 64 + lane]);
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[i], 0, 0, 0);
+                }
+            }
+        };
+        load(first);
+        leave(first);
+        load(first + 1);
         __syncthreads();
-        for (int un = first; un < last; ++un) {
-            const uint4 *keys = s_tile + ((un - first) & 1) * (KF + VF) * 64, *values = keys + KF * 64;
-            const int u0 = un * 64;
-            if (u0 < most) {
-                cf32x16 s[2];
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
-#pragma unroll
-                for (int i = 0; i < SK; ++i)
-#pragma unroll
-                    for (int tt = 0; tt < 2; ++tt) {
-                        const cb16x8 kf = __builtin_bit_cast(cb16x8, keys[(tt * SK + i) * 64 + lane]);
-#pragma unroll
-                        for (int k = 0; k < PQ; ++k) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], s[tt], 0, 0, 0);
-                    }
-                if (u0 + 64 > least) {
-#pragma unroll
-                    for (int r = 0; r < 32; ++r)
-                        if (u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3) >= lim) s[r >> 4][r & 15] = -INFINITY;
-                }
-                float top = s[0][0];
-#pragma unroll
-                for (int r = 1; r < 32; ++r) top = fmaxf(top, s[r >> 4][r & 15]);
-                if (__any(top > mx)) {
-                    const float now = fmaxf(mx, fmaxf(top, __shfl_xor(top, 32)));
-                    ref = now == -INFINITY ? 0.f : now * p.c2;
-                    const float shrink = __builtin_amdgcn_exp2f(fmaf(mx, p.c2, -ref));
-                    mx = now;
-                    sum *= shrink;
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) o[i] *= shrink;
-                }
-#pragma unroll
-                for (int sq = 0; sq < 4; ++sq) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = __builtin_amdgcn_exp2f(fmaf(s[sq >> 1][(sq & 1) * 8 + e], p.c2, -ref));
-                        sum += x[e];
-                    }
-                    cb16x8 pf[PP];
-                    split_pieces<PP>(x, pf);
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const cb16x8 vf = __builtin_bit_cast(cb16x8, values[(sq * NB + i) * 64 + lane]);
-#pragma unroll
-                        for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[i], 0, 0, 0);
-                    }
-                }
-            }
-            if (un + 1 < last) {
-                uint4 *to = s_tile + ((un + 1 - first) & 1) * (KF + VF) * 64;
-                store_tile<NB>(t, to, to + KF * 64, lane, wave);
-                at.load(min(un + 2, last - 1) * 64, t);
-            }
-            __syncthreads();
+        // Tiles that every row of the workgroup sees whole, then those on the border.  A step ends with the scores of the next
+        // tile, so that rescaling, a rare case, lies outside of the inner loops (inside, it cost 64 register copies a tile).
+        const int whole = max(first, min(last, least / TOKENS));
+        int un = first;
+        if (first < whole) product(un, std::false_type());
+        else product(un, std::true_type());
+        if (moved()) rescale();
+        while (un + 1 < whole) {
+            do {
+                apply(un);
+                ++un;
+                leave(un);
+                load(un + 1);
+                __syncthreads();
+                product(un, std::false_type());
+            } while (un + 1 < whole && !moved());
+            if (moved()) rescale();
         }
+        while (un + 1 < last) {
+            do {
+                apply(un);
+                ++un;
+                leave(un);
+                load(un + 1);
+                __syncthreads();
+                product(un, std::true_type());
+            } while (un + 1 < last && !moved());
+            if (moved()) rescale();
+        }
+        apply(un);
     }
     sum += __shfl_xor(sum, 32);
     if (row >= p.R) return;
-    const bool none = !real || mx == -INFINITY;
+    const bool none = !real || sum == 0.f;                        // (a row that sees nothing but NaN is NaN)
     const int tq = row / p.G, g = row - tq * p.G;
     if (p.nsplit > 1) {
         const long long gr = ((long long)split * bhs + bh) * p.R + row;
         float *to = p.part + gr * W;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
+        for (int r = 0; r < 16; ++r) {
+            float x[NB];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) to[(8 * (r >> 2) + 4 * l + (r & 3)) * NB + i] = o[i][r];
-        if (l == 0) p.part_ml[gr] = make_float2(none ? -INFINITY : ref, sum);
+            for (int i = 0; i < NB; ++i) x[i] = o[i][r];
+            store_n<CACHE_F32, NB>(to + (8 * (r >> 2) + 4 * l + (r & 3)) * NB, x);
+        }
+        if (l == 0) p.part_ml[gr] = make_float2(none ? -INFINITY : ref == -INFINITY ? 0.f : ref, sum);
         return;
     }
     const float inv = 1.f / sum;
@@ -849,12 +894,52 @@ __global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache
         for (int i = 0; i < NB; ++i) x[i] = none ? 0.f : o[i][r] * inv;
         store_n<DT, NB>(to + (long long)d * elem_bytes<DT>(), x);
     }
-    if (p.lse && l == 0) p.lse[bh * p.R + row] = none ? INFINITY : ref + __builtin_amdgcn_logf(sum);
+    if (p.lse && l == 0) p.lse[bh * p.R + row] = none ? INFINITY : (ref == -INFINITY ? 0.f : ref) + __builtin_amdgcn_logf(sum);
 }
 
-// Joins the pieces of a row, one workgroup a row: W / 8 lanes side by side in a piece, 2048 / W pieces at a time.  (One lane
-// group a row, walking over the pieces, took 152 us for 256 pieces of 32 rows: a chain of dependent loads.)
-constexpr int CACHE_MAX_SPLIT = 256;
+// Joins the pieces of a row: W / 8 lanes side by side in a piece.  More than 8 pieces: one workgroup a row, 2048 / W pieces at a time
+// (a lane group a row took 152 us for 256 pieces of 32 rows, a chain of dependent loads; this 6 us).  Otherwise a lane group a row
+// (65536 rows in 2 pieces, 128 wide: 72 us with a workgroup a row).
+constexpr int CACHE_MAX_SPLIT = 256, CACHE_FEW_SPLITS = 8;
+
+template <int DT, int W>
+__device__ __forceinline__ void store_joined(const CacheAttendParams &p, long long g0, int d, float (&x)[8], float big, float den)
+{
+    const float inv = 1.f / den;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = big == -INFINITY ? 0.f : x[i] * inv;
+    const long long bh = g0 / p.R;
+    const int row = (int)(g0 % p.R), b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads), t = row / p.G, g = row - t * p.G;
+    if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
+    if (p.lse && d == 0) p.lse[g0] = big == -INFINITY ? INFINITY : big + __builtin_amdgcn_logf(den);
+}
+
+template <int DT, int W>
+__global__ __launch_bounds__(256) void cache_join_few_kernel(CacheAttendParams p)
+{
+    const long long all = (long long)p.c.batch * p.c.heads * p.R, g0 = ((long long)blockIdx.x * 256 + threadIdx.x) / (W / 8);
+    const int d = threadIdx.x % (W / 8) * 8;
+    if (g0 >= all) return;
+    float2 ml[CACHE_FEW_SPLITS];
+    float big = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < CACHE_FEW_SPLITS; ++s) {
+        ml[s] = s < p.nsplit ? p.part_ml[s * all + g0] : make_float2(-INFINITY, 0.f);
+        big = fmaxf(big, ml[s].x);
+    }
+    float den = 0.f, x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < CACHE_FEW_SPLITS; ++s) {
+        if (ml[s].x == -INFINITY) continue;               // a piece that saw nothing has no sums to read
+        const float f = __builtin_amdgcn_exp2f(ml[s].x - big);
+        den += ml[s].y * f;
+        float y[8];
+        load8<CACHE_F32>(p.part + (s * all + g0) * W + d, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += y[i] * f;
+    }
+    store_joined<DT, W>(p, g0, d, x, big, den);
+}
 
 template <int DT, int W>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p)
@@ -902,13 +987,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p)
     for (int g = 1; g < GROUPS && g < p.nsplit; ++g)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] += s_x[g][d + i];
-    const float inv = 1.f / den;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = big == -INFINITY ? 0.f : x[i] * inv;
-    const long long bh = g0 / p.R;
-    const int row = (int)(g0 % p.R), b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads), t = row / p.G, g = row - t * p.G;
-    if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-    if (p.lse && d == 0) p.lse[g0] = big == -INFINITY ? INFINITY : big + __builtin_amdgcn_logf(den);
+    store_joined<DT, W>(p, g0, d, x, big, den);
 }
 
 // Attention sums: weight[slot] += sum over the query rows of exp(s - lse).  A wave has one unit of 32 bank rows and goes over
@@ -962,16 +1041,17 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
     }
 }
 
-// The same for many query rows: a wave keeps 64 bank rows as operands and the workgroup's four waves share tiles of 32 query rows
-// through shared memory.  Where bank rows are few, the query rows are cut into `rsplit` pieces, whose sums are added up after.
+// The same for many query rows: each of a workgroup's eight waves keeps 32 bank rows as operands, and all go over the query rows in
+// tiles of 64 that they share through shared memory.  Where bank rows are few, the query rows are cut into `rsplit` pieces, whose
+// sums are added up after.  What bounds it is the exponential: three vector instructions a score beside 8 / 32 of a matrix one
+// (1000 rows of 16 heads on 16 000: 255 us with 64 bank rows a wave and two waves a SIMD, which waited for their query rows).
 template <int DT, int NB>
-__global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_weigh_tile_kernel(CacheAttendParams p)
+__global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendParams p)
 {
-    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, MINE = SK / 4;      // steps of a query tile that a wave loads: NB / 2
-    static_assert(MINE * 4 == SK, "four waves");
-    __shared__ uint4 s_q[2][SK * PQ][64];
-    __shared__ float s_lse[2][32];
-    __shared__ int s_lim[2][32];
+    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, MINE = NB / 2;      // fragments of a query tile (2 SK) that a wave loads
+    constexpr int BUFS = 2 * SK * PQ > 64 ? 1 : 2;                // float32 at 256 dims: one buffer (96 KB) and a second barrier
+    __shared__ uint4 s_q[BUFS][2 * SK * PQ][64];
+    __shared__ float2 s_row[2][64];                               // log2 of the denominator, slots that the row sees
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
     const int bhs = p.c.batch * p.c.heads;
     const long long bh = blockIdx.x % bhs;
@@ -980,97 +1060,117 @@ __global__ __launch_bounds__(256, NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache
     int len = p.c.length[b];
     len = len > p.c.limit ? p.c.limit : len;
     const int n = real_rows(p.counts, b, p.T);
-    const int tiles = (int)(((long long)n * p.G + 31) / 32), per = (tiles + p.rsplit - 1) / p.rsplit;
+    const int tiles = (int)(((long long)n * p.G + 63) / 64), per = (tiles + p.rsplit - 1) / p.rsplit;
+    const char *const query = p.q + b * p.q_s[0] + (long long)h * p.G * p.q_s[1];
+    const int dt = 64 / p.G, dg = 64 - dt * p.G;                  // from a tile's row to the next one's, without a division
     for (int w0 = chunk * 256; w0 < len; w0 += p.chunks * 256) {
-        const int u0 = w0 + wave * 64;
-        cb16x8 kf[2][SK];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const long long at = min(u0 + 32 * tt + c, p.c.rows - 1);                // rows past the allocation: any row, left out below
-            const uint8_t *k = p.c.key + (bh * p.c.rows + at) * (W / 2) + l * (W / 4);
+        const int u0 = w0 + wave * 32;
+        cb16x8 kf[SK];
+        {
+            const long long at = min(u0 + c, p.c.rows - 1);       // rows past the allocation: any row, left out below
             uint32_t w[SK];
-            load_key<SK>(k, w);
+            load_key<SK>(p.c.key + (bh * p.c.rows + at) * (W / 2) + l * (W / 4), w);
 #pragma unroll
             for (int i = 0; i < SK; ++i) {
                 const uint32_t byte = p.c.key_scale[(bh * NB + (l * SK + i) / 4) * p.c.rows + at];
                 uint4 f = __builtin_bit_cast(uint4, cvt8(w[i], scale_of(byte)));
-                if (byte == 255) f = make_uint4(0x7fc07fc0u, 0, 0, 0);
-                kf[tt][i] = __builtin_bit_cast(cb16x8, f);
+                if (i == 0) f.x = byte == 255 ? 0x7fc07fc0u : f.x;
+                kf[i] = __builtin_bit_cast(cb16x8, f);
             }
         }
-        float w[32];
+        float w[16];
 #pragma unroll
-        for (int r = 0; r < 32; ++r) w[r] = 0.f;
+        for (int r = 0; r < 16; ++r) w[r] = 0.f;
         // tiles before the first row that sees slot w0 are left out
         const long long row_lo = (p.causal ? max(0, w0 - (len - n)) : 0) * (long long)p.G;
-        const int first = max(piece * per, (int)min((long long)tiles, row_lo / 32)), last = min(tiles, (piece + 1) * per);
+        const int first = max(piece * per, (int)min((long long)tiles, row_lo / 64)), last = min(tiles, (piece + 1) * per);
+        int next = first, t[2], g[2], row = first * 64 + lane;    // the tile that is loaded next; token and head of its rows c, 32 + c
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            t[a] = (first * 64 + 32 * a + c) / p.G;
+            g[a] = first * 64 + 32 * a + c - t[a] * p.G;
+        }
         uint4 mine[MINE * PQ];
-        float lse = 0.f;
-        int lim = 0;
-        const auto fetch = [&](int tile) {
-            const int row = tile * 32 + c;
-            const bool in = row < p.R && row / p.G < n;
-            lim = in ? visible(row / p.G, n, len, p.causal) : 0;
-            lse = lim > 0 ? p.lse[bh * p.R + row] : INFINITY;
+        float lse = INFINITY;
+        int sees = 0;
+        const auto fetch = [&]() {
+            if (next < last) {
+                const int tr = l ? t[1] : t[0];                   // row `lane` of the tile
+                sees = visible(tr, n, len, p.causal);
+                lse = sees > 0 ? p.lse[bh * p.R + row] : INFINITY;
 #pragma unroll
-            for (int m = 0; m < MINE; ++m) {
-                cb16x8 q[PQ];
-                load_query32<DT, NB, PQ>(p, b, h, in ? row : 0, l, lim > 0, wave * MINE + m, q);
+                for (int m = 0; m < MINE; ++m) {
+                    const int f = wave * MINE + m, a = f / SK, i = f % SK, d = l * 16 * NB + i * 8;
+                    const int ta = a ? t[1] : t[0], ga = a ? g[1] : g[0];
+                    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                    if (ta < n && d < p.c.dim) load8<DT>(query + (long long)ga * p.q_s[1] + ta * p.q_s[2] + (long long)d * elem_bytes<DT>(), x);
+                    cb16x8 q[PQ];
+                    split_pieces<PQ>(x, q);
 #pragma unroll
-                for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
+                    for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
+                }
+            }
+            ++next;
+            row += 64;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                t[a] += dt, g[a] += dg;
+                if (g[a] >= p.G) g[a] -= p.G, ++t[a];
             }
         };
         const auto leave = [&](int buf) {
 #pragma unroll
             for (int m = 0; m < MINE * PQ; ++m) s_q[buf][wave * MINE * PQ + m][lane] = mine[m];
-            if (wave == 0 && l == 0) s_lse[buf][c] = lse, s_lim[buf][c] = lim;
+            if (wave == 0) s_row[buf][lane] = make_float2(lse, __int_as_float(sees));
         };
         __syncthreads();
-        if (first < last) {
-            fetch(first);
-            leave(0);
-            fetch(min(first + 1, last - 1));
-        }
+        fetch();
+        leave(0);
+        fetch();
         __syncthreads();
         for (int tile = first; tile < last; ++tile) {
-            const int buf = (tile - first) & 1;
+            const int buf = (tile - first) & (BUFS - 1);
             cf32x16 s[2];
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
+                for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
 #pragma unroll
             for (int i = 0; i < SK; ++i)
 #pragma unroll
-                for (int k = 0; k < PQ; ++k) {
-                    const cb16x8 q = __builtin_bit_cast(cb16x8, s_q[buf][i * PQ + k][lane]);
+                for (int k = 0; k < PQ; ++k)
 #pragma unroll
-                    for (int tt = 0; tt < 2; ++tt) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[tt][i], q, s[tt], 0, 0, 0);
-                }
-            const float off = s_lse[buf][c];
-            const int sees = s_lim[buf][c];
-            if (__all(sees >= u0 + 64)) {
+                    for (int a = 0; a < 2; ++a)
+                        s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], __builtin_bit_cast(cb16x8, s_q[buf][(a * SK + i) * PQ + k][lane]), s[a], 0, 0, 0);
+            const float2 one = s_row[buf][c], two = s_row[buf][32 + c];
+            const int see[2] = {__float_as_int(one.y), __float_as_int(two.y)};
+            const float off[2] = {-one.x, -two.x};
+            if (__all(min(see[0], see[1]) >= u0 + 32)) {
 #pragma unroll
-                for (int r = 0; r < 32; ++r) w[r] += __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], p.c2, -off));
+                for (int r = 0; r < 16; ++r)
+                    w[r] += __builtin_amdgcn_exp2f(fmaf(s[0][r], p.c2, off[0])) + __builtin_amdgcn_exp2f(fmaf(s[1][r], p.c2, off[1]));
             } else {
 #pragma unroll
-                for (int r = 0; r < 32; ++r) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[r >> 4][r & 15], p.c2, -off));
-                    w[r] += u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3) < sees ? x : 0.f;
-                }
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, off[a]));
+                        w[r] += u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[a] ? x : 0.f;
+                    }
             }
+            if constexpr (BUFS == 1) __syncthreads();
             if (tile + 1 < last) {
-                leave(buf ^ 1);
-                fetch(min(tile + 2, last - 1));
+                leave(buf ^ (BUFS - 1));
+                fetch();
             }
             __syncthreads();
         }
         float *to = p.rsplit > 1 ? p.part_w + ((long long)piece * bhs + bh) * p.c.rows : p.c.weight + bh * p.c.rows;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
+        for (int r = 0; r < 16; ++r) {
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) w[r] += __shfl_xor(w[r], d);
-            const int slot = u0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * l + (r & 3);
+            const int slot = u0 + 8 * (r >> 2) + 4 * l + (r & 3);
             if (c == r && slot < len) {
                 if (p.rsplit > 1) to[slot] = w[r];
                 else to[slot] += w[r];

@@ -71,26 +71,54 @@ int check_grid(const char *who, int64_t blocks)
 // there are few of them.
 struct AttendPlan {
     int64_t R, mt, tiles, nsplit;
-    bool tiled;                              // 128 query rows a workgroup through shared memory, not 16 mt straight from memory
+    bool tiled;                              // 32 `waves` query rows a workgroup through shared memory, not 16 mt straight from memory
+    int waves;
     int64_t chunks, rsplit;                  // weights: workgroups a (sequence, head) along the bank, and along the query rows
     bool scores;                             // weights: from scores left behind, not from a second product
     size_t off_ml, off_lse, off_scores, off_w, total;
 };
 
-AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
+// How long the tiled form takes, in tiles of 128 rows of the bank by 256 query rows on one compute unit, with `waves` waves a
+// workgroup and the bank in `nsplit` pieces: the larger of an even share and the longest piece where pieces differ (causal, mostly
+// its own rows), whole rounds of equal pieces otherwise.  Measured: a workgroup of four waves (two a unit) needs 1 / 0.9 of the time
+// of one of eight for the same work; a tile is 3.8 us; getting started and leaving costs about 1.3 of them; joining pieces one, and
+// the writing and reading of their sums.
+double tiled_cost(int64_t bh, int64_t R, int width, int64_t span, double seen, bool uneven, int waves, int64_t nsplit)
+{
+    const int64_t tiles = ceil_div(R, 32 * waves), units = ceil_div(span, 16 * waves), per = ceil_div(units, nsplit);
+    const double slots = waves == 8 ? 256 : 512, unit = waves == 8 ? 1.0 : 0.5 / 0.9, over = 1.3;
+    const double share = seen / (double)span, groups = (double)(bh * tiles);
+    double t;
+    if (uneven) t = std::max(groups * ((double)units * share * unit + over * std::max(1.0, (double)nsplit * share)) / slots, (double)per * unit + over);
+    else t = ceil(groups * (double)nsplit / slots) * ((double)per * unit + over);
+    return t + (nsplit > 1 ? 1.0 + (double)(bh * R * nsplit) * width * 8 / (4.5e12 * 3.8e-6) : 0.0);
+}
+
+AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group, int64_t span, int causal, int accumulate)
 {
     AttendPlan a{};
     a.R = T * group;
     a.mt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
     const int64_t wide = (width_of(c->dim) == 256 ? 2 : 4) / (dtype == MI_F32 ? 2 : 1);      // what the register file holds
     if (a.mt > wide) a.mt = wide;
-    a.tiled = a.R >= 64;
-    a.tiles = ceil_div(a.R, a.tiled ? 128 : 16 * a.mt);
-    const int64_t bh = c->batch * c->heads, groups = bh * a.tiles;
+    const int64_t bh = c->batch * c->heads;
     span = span < 1 ? 1 : span > c->limit ? c->limit : span;
-    int64_t ns = ceil_div(a.tiled ? 512 : 768, groups);
-    const int64_t most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
-    a.nsplit = ns < 1 ? 1 : ns > most ? most : ns;
+    a.tiled = a.R >= 64;
+    if (a.tiled) {
+        const double seen = causal ? std::max((double)span * 0.5, (double)span - (double)T * 0.5) : (double)span;
+        const int64_t most = std::min<int64_t>(ceil_div(span, 256), mi::CACHE_MAX_SPLIT);
+        double best = 1e300;
+        for (int waves = dtype == MI_BF16 && width_of(c->dim) < 256 ? 8 : 4; waves >= 4; waves -= 4)
+            for (int64_t ns = 1; ns <= most; ++ns) {
+                const double t = tiled_cost(bh, a.R, width_of(c->dim), span, seen, causal && 2 * T > span, waves, ns);
+                if (t < best) best = t, a.waves = waves, a.nsplit = ns;
+            }
+        a.tiles = ceil_div(a.R, 32 * a.waves);
+    } else {
+        a.tiles = ceil_div(a.R, 16 * a.mt);
+        const int64_t ns = ceil_div(768, bh * a.tiles), most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
+        a.nsplit = ns > most ? most : ns;
+    }
     const int64_t rows = c->batch * c->heads * a.R;
     size_t at = 0;
     if (a.nsplit > 1) {
@@ -118,27 +146,42 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     return a;
 }
 
+template <int DT, int NB, int WAVES, bool EXACT>
+hipError_t launch_tile(const mi::CacheAttendParams &p, dim3 grid, hipStream_t s)
+{
+    const size_t lds = (size_t)NB * WAVES * 4 * 1024;      // two tiles of 16 WAVES rows, keys and values in bf16
+    static std::atomic<uint64_t> done{0};
+    const hipError_t e = ensure_dynamic_lds(mi::cache_attend_tile_kernel<DT, NB, WAVES, EXACT>, lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((mi::cache_attend_tile_kernel<DT, NB, WAVES, EXACT>), grid, dim3(64 * WAVES), lds, s, p);
+    return hipGetLastError();
+}
+
 template <int DT, int NB>
 hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, int accumulate, hipStream_t s)
 {
     const int64_t bh = (int64_t)p.c.batch * p.c.heads;
     const dim3 grid((unsigned)(bh * a.tiles * a.nsplit));
     if (a.tiled) {
-        const size_t lds = (size_t)NB * 16 * 1024;         // two tiles of 64 rows, keys and values in bf16
-        static std::atomic<uint64_t> done{0};
-        const hipError_t e = ensure_dynamic_lds(mi::cache_attend_tile_kernel<DT, NB>, lds, done);
+        hipError_t e;
+        if constexpr (DT == mi::CACHE_BF16) {
+            if constexpr (NB < 8) e = a.waves == 8 ? (accumulate ? launch_tile<DT, NB, 8, true>(p, grid, s) : launch_tile<DT, NB, 8, false>(p, grid, s))
+                                                   : (accumulate ? launch_tile<DT, NB, 4, true>(p, grid, s) : launch_tile<DT, NB, 4, false>(p, grid, s));
+            else e = accumulate ? launch_tile<DT, NB, 4, true>(p, grid, s) : launch_tile<DT, NB, 4, false>(p, grid, s);
+        } else e = launch_tile<DT, NB, 4, true>(p, grid, s);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((mi::cache_attend_tile_kernel<DT, NB>), grid, dim3(256), lds, s, p);
     } else if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
     if constexpr (NB < 8 || DT != mi::CACHE_F32)
         if (!a.tiled && a.mt == 2) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 2>), grid, dim3(256), 0, s, p);
     if constexpr (NB < 8 && DT != mi::CACHE_F32)
         if (!a.tiled && a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
-    if (a.nsplit > 1)
+    if (a.nsplit > 1 && a.nsplit <= mi::CACHE_FEW_SPLITS)
+        hipLaunchKernelGGL((mi::cache_join_few_kernel<DT, 32 * NB>), dim3((unsigned)ceil_div(bh * a.R * (4 * NB), 256)), dim3(256), 0, s, p);
+    else if (a.nsplit > 1)
         hipLaunchKernelGGL((mi::cache_join_kernel<DT, 32 * NB>), dim3((unsigned)(bh * a.R)), dim3(256), 0, s, p);
     if (a.scores) hipLaunchKernelGGL(mi::cache_weigh_scores_kernel, dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
     else if (accumulate && a.tiled) {
-        hipLaunchKernelGGL((mi::cache_weigh_tile_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks * a.rsplit)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((mi::cache_weigh_tile_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks * a.rsplit)), dim3(512), 0, s, p);
         if (a.rsplit > 1) hipLaunchKernelGGL(mi::cache_weigh_add_kernel, dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
     } else if (accumulate) hipLaunchKernelGGL((mi::cache_weigh_kernel<DT, NB>), dim3((unsigned)(bh * a.chunks)), dim3(256), 0, s, p);
     return hipGetLastError();
@@ -223,10 +266,10 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
     return MI_OK;
 }
 
-size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int accumulate)
+size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int causal, int accumulate)
 {
     if (check_cache(cache, "mi_cache_attend_workspace_bytes") || !known_dtype(dtype) || T < 1 || group < 1 || group > 65536 || T > MAX_ROWS / group) return 0;
-    return attend_plan(cache, dtype, T, group, span, accumulate).total;
+    return attend_plan(cache, dtype, T, group, span, causal, accumulate).total;
 }
 
 int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *query_strides, void *out, const int64_t *out_strides,
@@ -241,7 +284,7 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     mi::CacheAttendParams p{};
     MI_TRY(check_rows("mi_cache_attend", "query", query, query_strides, dtype, p.q_s));
     MI_TRY(check_rows("mi_cache_attend", "out", out, out_strides, dtype, p.out_s));
-    const AttendPlan a = attend_plan(cache, dtype, T, group, span, accumulate);
+    const AttendPlan a = attend_plan(cache, dtype, T, group, span, causal, accumulate);
     if (!workspace || ((uintptr_t)workspace & 15)) return fail(MI_ERR_ARG, "mi_cache_attend: workspace must be 16-byte aligned");
     if (workspace_bytes < a.total) return fail(MI_ERR_WORKSPACE, "mi_cache_attend: workspace %zu < required %zu", workspace_bytes, a.total);
     const int width = width_of(cache->dim);

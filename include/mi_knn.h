@@ -231,7 +231,8 @@ int mi_queue_push_stash(void *queue, int64_t K, int64_t row_bytes, int64_t ptr,
  * Format: a row of `dim` values, zero padded to `width` = 64, 128 or 256, in blocks of 32.  A block has one scale 2^e, e the
  * smallest integer with max|x| <= 7 * 2^e, clamped to [-126, 125], held as the byte e + 127; elements are x / 2^e rounded to
  * nearest (ties to even, saturating) on 0 0.5 1 1.5 2 3 4 6 with a sign bit, two a byte, the even one in the low four bits.
- * A row of a head with a NaN or an infinity in its key or its value is held as NaN whole (all scale bytes 255, elements 0).
+ * A row of a head with a NaN or an infinity in its key or its value is held as NaN whole: scale bytes 255 on the key and 0 on
+ * the value, elements 0.
  * All pointers are device memory, 16-byte aligned; `rows` (allocated) is a multiple of 64, `limit` <= rows the most in use. */
 typedef struct {
     uint8_t *key, *key_scale;        /* [batch][heads][rows][width / 2], [batch][heads][width / 32][rows] */
@@ -268,7 +269,7 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
  * query, out: [batch][heads * group][T][dim] of `dtype` with strides as in mi_cache_push.  Products are exact in bf16 pieces of
  * the query (one for bf16, two for float16, three for float32), sums and softmax statistics are float32.
  * `span`: about how many rows are in use (it sizes the launch; the result is right for any span >= 1). */
-size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int accumulate);
+size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int causal, int accumulate);
 int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *query_strides, void *out, const int64_t *out_strides,
                     int dtype, int64_t T, int64_t group, const int32_t *counts, float scale, int causal, int accumulate, int64_t span,
                     void *workspace, size_t workspace_bytes, mi_stream_t stream);

@@ -133,8 +133,8 @@ def test_abi_refuses_bad_calls_before_touching_the_device():
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert attend(scale=scale) == -1 and b"scale" in L.mi_last_error()
     assert attend(ws=None) == -1 and attend(nbytes=1) == -3 and attend(group=0) == -1 and attend(T=-1) == -1 and attend(dtype=3) == -1 and attend(out=None) == -1
-    assert L.mi_cache_attend_workspace_bytes(cache(), 1, 0, 1, 10, 0) == 0 and L.mi_cache_attend_workspace_bytes(cache(), 9, 1, 1, 10, 0) == 0
-    assert L.mi_cache_attend_workspace_bytes(cache(), 1, 1, 1, 10, 0) > 0
+    assert L.mi_cache_attend_workspace_bytes(cache(), 1, 0, 1, 10, 1, 0) == 0 and L.mi_cache_attend_workspace_bytes(cache(), 9, 1, 1, 10, 1, 0) == 0
+    assert L.mi_cache_attend_workspace_bytes(cache(), 1, 1, 1, 10, 1, 0) > 0
     assert L.mi_cache_evict_workspace_bytes(cache(), 10) >= 4 * 10 * 8 and L.mi_cache_evict_workspace_bytes(cache(), 0) == 0
 
     def evict(into=None, keep=10, recent=0, ws=at, nbytes=1 << 30):
@@ -269,7 +269,7 @@ def _filled(rs, B, H, dim, k, fill, dtype="bf16", spread=0.7):
 @gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("dim,H,group,T,fill", [(64, 1, 1, 1, 1), (64, 2, 1, 1, 31), (128, 2, 4, 1, 33), (72, 1, 3, 1, 257), (256, 2, 2, 1, 700), (128, 1, 16, 1, 1500),
-                                                (128, 1, 17, 1, 300), (64, 1, 2, 9, 65), (160, 2, 1, 5, 129), (128, 1, 4, 40, 40), (96, 1, 1, 70, 200), (256, 1, 3, 50, 128), (8, 1, 1, 200, 513)])
+                                                (128, 1, 17, 1, 300), (64, 1, 2, 9, 65), (160, 2, 1, 5, 129), (128, 1, 4, 40, 40), (96, 1, 1, 70, 200), (128, 1, 4, 70, 330), (64, 1, 3, 100, 640), (256, 1, 3, 50, 128), (8, 1, 1, 200, 513)])
 def test_attend_against_64_bits(dtype, dim, H, group, T, fill):
     rs = np.random.RandomState(dim + T + fill)
     B = 3
@@ -344,6 +344,18 @@ def test_attend_nan_rows_reach_only_who_sees_them():
         q = q[:, :, :20]
         out = bank.attend("kv", q.cuda(), causal=False)
         _check_out(out, *ref.attend(_np(q), causal=False), "fp32")
+
+
+@gpu
+@pytest.mark.parametrize("T,fill", [(1, 1), (1, 600), (70, 70), (200, 900)])
+def test_attend_rows_that_see_nothing_but_nan(T, fill):
+    kv = torch.full((1, 1, fill, 64), float("nan"), device="cuda")
+    bank = _bank(1, 1, 64, fill)
+    bank.push("kv", kv, kv)
+    q = torch.randn(1, 1, T, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(0))
+    for dtype in (torch.float32, torch.bfloat16):
+        out = bank.attend("kv", q.to(dtype), accumulate=True)
+        assert torch.isnan(out).all() and torch.isnan(bank.weights("kv")).all()
 
 
 @gpu
