@@ -767,13 +767,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
         const TileAt<NB> at(p.c, bh, lane, wave & 3);
         TileRegs<NB> t;
         // four waves have 64 rows of a tile; where those lie past the allocation (a multiple of 64), its last 64 stand in: they are masked
-        const auto load = [&](int un) { at.load(min(min(un, last - 1) * TOKENS + 64 * (wave >> 2), p.c.rows - 64), t); };
-        const auto leave = [&](int un) {
+        const auto load = [&](int un) __attribute__((always_inline)) { at.load(min(min(un, last - 1) * TOKENS + 64 * (wave >> 2), p.c.rows - 64), t); };
+        const auto leave = [&](int un) __attribute__((always_inline)) {
             uint4 *to = s_tile + ((un - first) & 1) * (KF + VF) * 64;
             store_tile<NB>(t, to, to + KF * 64, lane, wave);
         };
         // scores of a tile and the largest of them
-        const auto product = [&](int un, auto masked) {
+        const auto product = [&](int un, auto masked) __attribute__((always_inline)) {
             const uint4 *keys = s_tile + ((un - first) & 1) * (KF + VF) * 64;
 #pragma unroll
             for (int tt = 0; tt < SUB; ++tt)
@@ -797,8 +797,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
 #pragma unroll
             for (int r = 1; r < 16 * SUB; ++r) top = fmaxf(top, s[r >> 4][r & 15]);
         };
-        const auto moved = [&]() { return __any(fmaf(top, p.c2, -CACHE_SLACK) > ref); };
-        const auto rescale = [&]() {
+        const auto moved = [&]() __attribute__((always_inline)) { return __any(fmaf(top, p.c2, -CACHE_SLACK) > ref); };
+        const auto rescale = [&]() __attribute__((always_inline)) {
             const float now = fmaxf(ref, fmaxf(top, __shfl_xor(top, 32)) * p.c2);
             const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
             ref = now;
@@ -806,7 +806,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
 #pragma unroll
             for (int i = 0; i < NB; ++i) o[i] *= shrink;
         };
-        const auto apply = [&](int un) {
+        const auto apply = [&](int un) __attribute__((always_inline)) {
             const uint4 *values = s_tile + ((un - first) & 1) * (KF + VF) * 64 + KF * 64;
             const float off = ref == -INFINITY ? 0.f : -ref;
 #pragma unroll
@@ -1042,16 +1042,17 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
 }
 
 // The same for many query rows: each of a workgroup's eight waves keeps 32 bank rows as operands, and all go over the query rows in
-// tiles of 64 that they share through shared memory.  Where bank rows are few, the query rows are cut into `rsplit` pieces, whose
-// sums are added up after.  What bounds it is the exponential: three vector instructions a score beside 8 / 32 of a matrix one
-// (1000 rows of 16 heads on 16 000: 255 us with 64 bank rows a wave and two waves a SIMD, which waited for their query rows).
+// tiles of 64 that they share through shared memory.  The scores of a tile are computed while the exponentials of the one before
+// are: what bounds it is three vector instructions a score beside 8 / 32 of a matrix one.  Where bank rows are few, the query rows
+// are cut into `rsplit` pieces, whose sums are added up after.  (1000 rows of 16 heads on 16 000: 255 us with 64 bank rows a wave,
+// 207 us with tiles of 32 and four waves a SIMD, in both each wave's products and exponentials in turn.)
 template <int DT, int NB>
 __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendParams p)
 {
-    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, MINE = NB / 2;      // fragments of a query tile (2 SK) that a wave loads
-    constexpr int BUFS = 2 * SK * PQ > 64 ? 1 : 2;                // float32 at 256 dims: one buffer (96 KB) and a second barrier
-    __shared__ uint4 s_q[BUFS][2 * SK * PQ][64];
-    __shared__ float2 s_row[2][64];                               // log2 of the denominator, slots that the row sees
+    constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, RT = 2 * SK * PQ > 64 ? 1 : 2, QROWS = 32 * RT;
+    constexpr int MINE = RT * SK / 8;                             // fragments of a query tile (RT SK) that a wave loads
+    static_assert(MINE * 8 == RT * SK, "eight waves");
+    __shared__ uint4 s_q[2][RT * SK * PQ][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
     const int bhs = p.c.batch * p.c.heads;
     const long long bh = blockIdx.x % bhs;
@@ -1060,9 +1061,9 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
     int len = p.c.length[b];
     len = len > p.c.limit ? p.c.limit : len;
     const int n = real_rows(p.counts, b, p.T);
-    const int tiles = (int)(((long long)n * p.G + 63) / 64), per = (tiles + p.rsplit - 1) / p.rsplit;
+    const int tiles = (int)(((long long)n * p.G + QROWS - 1) / QROWS), per = (tiles + p.rsplit - 1) / p.rsplit;
     const char *const query = p.q + b * p.q_s[0] + (long long)h * p.G * p.q_s[1];
-    const int dt = 64 / p.G, dg = 64 - dt * p.G;                  // from a tile's row to the next one's, without a division
+    const int dt = QROWS / p.G, dg = QROWS - dt * p.G;            // from a tile's row to the next one's, without a division
     for (int w0 = chunk * 256; w0 < len; w0 += p.chunks * 256) {
         const int u0 = w0 + wave * 32;
         cb16x8 kf[SK];
@@ -1081,89 +1082,113 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
         float w[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) w[r] = 0.f;
-        // tiles before the first row that sees slot w0 are left out
-        const long long row_lo = (p.causal ? max(0, w0 - (len - n)) : 0) * (long long)p.G;
-        const int first = max(piece * per, (int)min((long long)tiles, row_lo / 64)), last = min(tiles, (piece + 1) * per);
-        int next = first, t[2], g[2], row = first * 64 + lane;    // the tile that is loaded next; token and head of its rows c, 32 + c
+        // tiles before the first row that sees slot w0 are left out; those before the first that sees all slots of the workgroup
+        // are masked (rows that are not real divide by infinity)
+        const int t_lo = p.causal ? max(0, w0 - (len - n)) : 0, t_all = p.causal ? max(0, w0 + 255 - (len - n)) : 0;
+        const int first = max(piece * per, (int)min((long long)tiles, (long long)t_lo * p.G / QROWS)), last = min(tiles, (piece + 1) * per);
+        const int border = max(first, (int)min((long long)last, ((long long)t_all * p.G + QROWS - 1) / QROWS));
+        if (first < last) {
+            int t[RT], g[RT];                                     // token and head of rows c, 32 + c of the tile that is loaded next
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            t[a] = (first * 64 + 32 * a + c) / p.G;
-            g[a] = first * 64 + 32 * a + c - t[a] * p.G;
-        }
-        uint4 mine[MINE * PQ];
-        float lse = INFINITY;
-        int sees = 0;
-        const auto fetch = [&]() {
-            if (next < last) {
-                const int tr = l ? t[1] : t[0];                   // row `lane` of the tile
-                sees = visible(tr, n, len, p.causal);
-                lse = sees > 0 ? p.lse[bh * p.R + row] : INFINITY;
+            for (int a = 0; a < RT; ++a) {
+                t[a] = (first * QROWS + 32 * a + c) / p.G;
+                g[a] = first * QROWS + 32 * a + c - t[a] * p.G;
+            }
+            uint4 mine[MINE * PQ];
+            float off[3][RT];                                     // less the log2 of the denominator: of the tile in hand, the next, the one loaded
+            int see[3][RT];
+            const auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int a = 0; a < RT; ++a) {
+                    const bool real = t[a] < n;
+                    see[2][a] = real ? visible(t[a], n, len, p.causal) : 0;
+                    const float lse = p.lse[bh * p.R + (real ? t[a] * p.G + g[a] : 0)];
+                    off[2][a] = see[2][a] > 0 ? -lse : -INFINITY;
+                }
 #pragma unroll
                 for (int m = 0; m < MINE; ++m) {
-                    const int f = wave * MINE + m, a = f / SK, i = f % SK, d = l * 16 * NB + i * 8;
-                    const int ta = a ? t[1] : t[0], ga = a ? g[1] : g[0];
-                    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (ta < n && d < p.c.dim) load8<DT>(query + (long long)ga * p.q_s[1] + ta * p.q_s[2] + (long long)d * elem_bytes<DT>(), x);
-                    cb16x8 q[PQ];
-                    split_pieces<PQ>(x, q);
+                    const int f = wave * MINE + m, a = f / SK, d = l * 16 * NB + f % SK * 8;
+                    const int ta = a ? t[RT - 1] : t[0], ga = a ? g[RT - 1] : g[0];
+                    const bool in = ta < n && d < p.c.dim;
+                    const char *src = query + (in ? (long long)ga * p.q_s[1] + ta * p.q_s[2] + (long long)d * elem_bytes<DT>() : 0);
+                    if constexpr (DT == CACHE_BF16) {
+                        const uint4 x = *(const uint4 *)src;
+                        mine[m] = make_uint4(in ? x.x : 0, in ? x.y : 0, in ? x.z : 0, in ? x.w : 0);
+                    } else {
+                        float x[8];
+                        load8<DT>(src, x);
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
+                        for (int i = 0; i < 8; ++i) x[i] = in ? x[i] : 0.f;
+                        cb16x8 q[PQ];
+                        split_pieces<PQ>(x, q);
+#pragma unroll
+                        for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
+                    }
                 }
-            }
-            ++next;
-            row += 64;
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                t[a] += dt, g[a] += dg;
-                if (g[a] >= p.G) g[a] -= p.G, ++t[a];
-            }
-        };
-        const auto leave = [&](int buf) {
+                for (int a = 0; a < RT; ++a) {
+                    t[a] += dt, g[a] += dg;
+                    if (g[a] >= p.G) g[a] -= p.G, ++t[a];
+                }
+            };
+            const auto leave = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-            for (int m = 0; m < MINE * PQ; ++m) s_q[buf][wave * MINE * PQ + m][lane] = mine[m];
-            if (wave == 0) s_row[buf][lane] = make_float2(lse, __int_as_float(sees));
-        };
-        __syncthreads();
-        fetch();
-        leave(0);
-        fetch();
-        __syncthreads();
-        for (int tile = first; tile < last; ++tile) {
-            const int buf = (tile - first) & (BUFS - 1);
-            cf32x16 s[2];
+                for (int m = 0; m < MINE * PQ; ++m) s_q[(tile - first) & 1][wave * MINE * PQ + m][lane] = mine[m];
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < RT; ++a) off[0][a] = off[1][a], off[1][a] = off[2][a], see[0][a] = see[1][a], see[1][a] = see[2][a];
+            };
+            const auto product = [&](int tile, cf32x16 (&s)[RT]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
+                for (int a = 0; a < RT; ++a)
 #pragma unroll
-            for (int i = 0; i < SK; ++i)
+                    for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
 #pragma unroll
-                for (int k = 0; k < PQ; ++k)
+                for (int i = 0; i < SK; ++i)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a)
-                        s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], __builtin_bit_cast(cb16x8, s_q[buf][(a * SK + i) * PQ + k][lane]), s[a], 0, 0, 0);
-            const float2 one = s_row[buf][c], two = s_row[buf][32 + c];
-            const int see[2] = {__float_as_int(one.y), __float_as_int(two.y)};
-            const float off[2] = {-one.x, -two.x};
-            if (__all(min(see[0], see[1]) >= u0 + 32)) {
+                    for (int k = 0; k < PQ; ++k)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    w[r] += __builtin_amdgcn_exp2f(fmaf(s[0][r], p.c2, off[0])) + __builtin_amdgcn_exp2f(fmaf(s[1][r], p.c2, off[1]));
-            } else {
+                        for (int a = 0; a < RT; ++a)
+                            s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], __builtin_bit_cast(cb16x8, s_q[(tile - first) & 1][(a * SK + i) * PQ + k][lane]), s[a], 0, 0, 0);
+            };
+            // scores of the next tile (past the last one: of whatever is there, never used) beside the exponentials of this one
+            const auto step = [&](int tile, cf32x16 (&s)[RT], cf32x16 (&ahead)[RT], auto masked) __attribute__((always_inline)) {
+                product(tile + 1, ahead);
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < RT; ++a)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, off[a]));
-                        w[r] += u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[a] ? x : 0.f;
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, off[0][a]));
+                        if constexpr (decltype(masked)::value) w[r] += u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[0][a] ? x : 0.f;
+                        else w[r] += x;
                     }
-            }
-            if constexpr (BUFS == 1) __syncthreads();
-            if (tile + 1 < last) {
-                leave(buf ^ (BUFS - 1));
+                leave(tile);                                      // tile + 2, into the buffer that this tile had
                 fetch();
-            }
+                __syncthreads();
+            };
+            cf32x16 s0[RT], s1[RT];
+            int tile = first;
+            const auto run = [&](int end, auto masked) __attribute__((always_inline)) {
+                for (; tile + 1 < end; tile += 2) {
+                    step(tile, s0, s1, masked);
+                    step(tile + 1, s1, s0, masked);
+                }
+                if (tile < end) {
+                    step(tile, s0, s1, masked);
+                    ++tile;
+#pragma unroll
+                    for (int a = 0; a < RT; ++a) s0[a] = s1[a];
+                }
+            };
             __syncthreads();
+            fetch();
+            leave(first);
+            fetch();
+            leave(first + 1);
+            fetch();
+            __syncthreads();
+            product(first, s0);
+            run(border, std::true_type());
+            run(last, std::false_type());
         }
         float *to = p.rsplit > 1 ? p.part_w + ((long long)piece * bhs + bh) * p.c.rows : p.c.weight + bh * p.c.rows;
 #pragma unroll

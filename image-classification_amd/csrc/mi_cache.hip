@@ -89,7 +89,7 @@ double tiled_cost(int64_t bh, int64_t R, int width, int64_t span, double seen, b
     const double slots = waves == 8 ? 256 : 512, unit = waves == 8 ? 1.0 : 0.5 / 0.9, over = 1.3;
     const double share = seen / (double)span, groups = (double)(bh * tiles);
     double t;
-    if (uneven) t = std::max(groups * ((double)units * share * unit + over * std::max(1.0, (double)nsplit * share)) / slots, (double)per * unit + over);
+    if (uneven) t = std::max(groups * ((double)units * share * unit + over * std::max(1.0, (double)nsplit * share)) / slots, (double)per * unit * (waves == 8 ? 1.0 : 0.8) + over);
     else t = ceil(groups * (double)nsplit / slots) * ((double)per * unit + over);
     return t + (nsplit > 1 ? 1.0 + (double)(bh * R * nsplit) * width * 8 / (4.5e12 * 3.8e-6) : 0.0);
 }
