@@ -1187,6 +1187,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
             fetch();
             __syncthreads();
             product(first, s0);
+            __syncthreads();                                      // the first step writes where this one read
             run(border, std::true_type());
             run(last, std::false_type());
         }
