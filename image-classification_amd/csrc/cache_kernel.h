@@ -458,11 +458,17 @@ __device__ __forceinline__ float across_j_sum(float x)
 // Streaming form: a workgroup has MT tiles of 16 query rows of one (sequence, head) and one piece of its bank rows; its four
 // waves take every fourth unit of 32 rows each, straight from memory into registers, and are joined at the end.
 template <int DT, int NB, int MT>
-__global__ __launch_bounds__(256, MT == 1 && NB < 8 ? 2 : 1) void cache_attend_kernel(CacheAttendParams p)
+__global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams p)
 {
     constexpr int W = 32 * NB, PQ = Pieces<DT>::N, PP = DT == CACHE_F32 ? 3 : 2, LD = W + 4;
+    // Query operands stay in registers where they fit beside the sums of two waves a SIMD, else in shared memory, which the sums of
+    // the four waves use after the loop.
+    constexpr bool Q_LDS = NB == 8 || MT * NB * (PQ + 2) >= 32;
+    constexpr bool TIGHT = MT * NB >= 8;     // conversions stay with their product: moved ahead of it by the scheduler they spill
+    constexpr int O_BYTES = 4 * 16 * LD * 4, Q_BYTES = Q_LDS ? MT * NB * PQ * 1024 : 0;
     __shared__ float s_m[4][16], s_l[4][16];
-    __shared__ float s_o[4][16][LD];
+    __shared__ alignas(16) char s_both[O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES];
+    float (&s_o)[4][16][LD] = *(float (*)[4][16][LD])s_both;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
     long long id = blockIdx.x;
     const int split = (int)(id % p.nsplit);
@@ -474,14 +480,22 @@ __global__ __launch_bounds__(256, MT == 1 && NB < 8 ? 2 : 1) void cache_attend_k
     len = len > p.c.limit ? p.c.limit : len;
     const int n = real_rows(p.counts, b, p.T);
 
-    cb16x8 q[MT][NB][PQ];
+    cb16x8 q[Q_LDS ? 1 : MT][NB][PQ];
     int lim[MT], most = 0, least = 0x7fffffff;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int row = (tile * MT + m) * 16 + c;
         const bool in = row < p.R;
         lim[m] = in ? visible(row / p.G, n, len, p.causal) : 0;
-        load_query<DT, NB, PQ>(p, b, h, in ? row : 0, j, lim[m] > 0, q[m]);
+        load_query<DT, NB, PQ>(p, b, h, in ? row : 0, j, lim[m] > 0, q[Q_LDS ? 0 : m]);
+        if constexpr (Q_LDS) {                                    // every wave has them all: each leaves a quarter
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (i % 4 == wave % 4 || NB < 4) {
+#pragma unroll
+                    for (int k = 0; k < PQ; ++k) ((uint4 *)s_both)[((m * NB + i) * PQ + k) * 64 + lane] = __builtin_bit_cast(uint4, q[0][i][k]);
+                }
+        }
         most = max(most, lim[m]);
         least = min(least, lim[m]);
     }
@@ -507,26 +521,30 @@ __global__ __launch_bounds__(256, MT == 1 && NB < 8 ? 2 : 1) void cache_attend_k
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) o[m][i] = cf32x4{0, 0, 0, 0};
     }
+    if constexpr (Q_LDS) __syncthreads();
     const UnitAt<NB> at(p.c, bh, lane);
-    Unit<NB> next;
-    if (first + wave < last) at.load((first + wave) * 32, next);
-    for (int un = first + wave; un < last; un += 4) {
-        const int u0 = un * 32;
-        const Unit<NB> u = next;
-        at.load(min(un + 4, last - 1) * 32, next);        // the next unit is on its way while this one is computed
+    const auto query = [&](int m, int i, int k) __attribute__((always_inline)) {
+        if constexpr (Q_LDS) return __builtin_bit_cast(cb16x8, ((const uint4 *)s_both)[((m * NB + i) * PQ + k) * 64 + lane]);
+        else return q[m][i][k];
+    };
+    const auto compute = [&](int u0, const Unit<NB> &u) __attribute__((always_inline)) {
         cf32x4 s[MT][2];
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][a] = cf32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const cb16x8 kf = key_operand<NB>(u.k[a], u.ks[a], i);
+        for (int i = 0; i < NB; ++i) {
+            const cb16x8 kf[2] = {key_operand<NB>(u.k[0], u.ks[0], i), key_operand<NB>(u.k[1], u.ks[1], i)};
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k) s[m][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[m][i][k], s[m][a], 0, 0, 0);
-            }
+                for (int k = 0; k < PQ; ++k) {
+                    const cb16x8 qf = query(m, i, k);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) s[m][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], qf, s[m][a], 0, 0, 0);
+                }
+            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
         cb16x8 pf[MT][PP];
 #pragma unroll
@@ -582,10 +600,25 @@ __global__ __launch_bounds__(256, MT == 1 && NB < 8 ? 2 : 1) void cache_attend_k
                     o[m][2 * i2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, pf[m][k], o[m][2 * i2], 0, 0, 0);
                     o[m][2 * i2 + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, pf[m][k], o[m][2 * i2 + 1], 0, 0, 0);
                 }
+            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // DEPTH units are on their way or in hand: a unit is computed about as fast as memory answers
+    constexpr int DEPTH = MT * NB <= 4 ? 3 : NB < 8 && DT == CACHE_BF16 ? 2 : 1;
+    Unit<NB> u[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (first + wave + 4 * d < last) at.load((long long)(first + wave + 4 * d) * 32, u[d]);
+    for (int un = first + wave; un < last; un += 4 * DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (un + 4 * d >= last) break;
+            compute((un + 4 * d) * 32, u[d]);
+            if (un + 4 * (d + DEPTH) < last) at.load((long long)(un + 4 * (d + DEPTH)) * 32, u[d]);
         }
     }
 
-    // join the four waves, one tile of 16 rows at a time
+    // join the four waves, one tile of 16 rows at a time (what the loop read of shared memory is read: the barrier below)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const float l = across_j_sum(sum[m]);

@@ -98,12 +98,10 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
 {
     AttendPlan a{};
     a.R = T * group;
-    a.mt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-    const int64_t wide = (width_of(c->dim) == 256 ? 2 : 4) / (dtype == MI_F32 ? 2 : 1);      // what the register file holds
-    if (a.mt > wide) a.mt = wide;
+    a.mt = a.R <= 16 || width_of(c->dim) == 256 ? 1 : 2;         // 256 dims: the sums of two tiles do not fit two waves a SIMD
     const int64_t bh = c->batch * c->heads;
     span = span < 1 ? 1 : span > c->limit ? c->limit : span;
-    a.tiled = a.R >= 64;
+    a.tiled = a.R > 32;
     if (a.tiled) {
         const double seen = causal ? std::max((double)span * 0.5, (double)span - (double)T * 0.5) : (double)span;
         const int64_t most = std::min<int64_t>(ceil_div(span, 256), mi::CACHE_MAX_SPLIT);
@@ -171,10 +169,8 @@ hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, in
         } else e = launch_tile<DT, NB, 4, true>(p, grid, s);
         if (e != hipSuccess) return e;
     } else if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
-    if constexpr (NB < 8 || DT != mi::CACHE_F32)
+    if constexpr (NB < 8)
         if (!a.tiled && a.mt == 2) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 2>), grid, dim3(256), 0, s, p);
-    if constexpr (NB < 8 && DT != mi::CACHE_F32)
-        if (!a.tiled && a.mt == 4) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 4>), grid, dim3(256), 0, s, p);
     if (a.nsplit > 1 && a.nsplit <= mi::CACHE_FEW_SPLITS)
         hipLaunchKernelGGL((mi::cache_join_few_kernel<DT, 32 * NB>), dim3((unsigned)ceil_div(bh * a.R * (4 * NB), 256)), dim3(256), 0, s, p);
     else if (a.nsplit > 1)
