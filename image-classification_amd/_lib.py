@@ -18,7 +18,7 @@ EXPORTS = [
     "mi_abi_version", "mi_last_error", "mi_profile_enable", "mi_profile_collect", "mi_profile_clock", "mi_debug_force_fallback", "mi_knn_ld", "mi_pack_rows", "mi_knn_topk_workspace_bytes", "mi_knn_topk_workspace_bytes_for_budget",
     "mi_knn_topk", "mi_knn_topk_static", "mi_knn_merge", "mi_knn_vote", "mi_queue_push", "mi_bank_scatter", "mi_moco_workspace_bytes",
     "mi_moco_fwd", "mi_moco_bwd", "mi_queue_push_stash", "mi_bank_append_normalized", "mi_queue_push_wrap", "mi_soft_knn_workspace_bytes", "mi_soft_knn", "mi_kth_largest",
-    "mi_cache_width", "mi_cache_push", "mi_cache_trim", "mi_cache_read", "mi_cache_attend_workspace_bytes", "mi_cache_attend",
+    "mi_cache_width", "mi_cache_push", "mi_cache_longest", "mi_cache_trim", "mi_cache_read", "mi_cache_attend_workspace_bytes", "mi_cache_attend",
     "mi_cache_evict_workspace_bytes", "mi_cache_evict",
 ]
 
@@ -94,6 +94,7 @@ def lib() -> ctypes.CDLL:
     L.mi_cache_width.restype, L.mi_cache_width.argtypes = i64, [i64]
     L.mi_cache_push.restype = i32
     L.mi_cache_push.argtypes = [cache, p, strides, p, strides, i32, i64, p, p, p, p]
+    L.mi_cache_longest.restype, L.mi_cache_longest.argtypes = i32, [cache, p, i64, p, p]
     L.mi_cache_trim.restype, L.mi_cache_trim.argtypes = i32, [cache, p, i64, p]
     L.mi_cache_read.restype, L.mi_cache_read.argtypes = i32, [cache, p, p, p]
     L.mi_cache_attend_workspace_bytes.restype = sz
@@ -121,6 +122,13 @@ def check(rc: int, what: str) -> None:
 def stream_ptr(device) -> int:
     import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """:func:`stream_ptr` of device ``index`` without a Stream object around it (2 us less on a call of 15)."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def profile_enable(on: bool) -> None:

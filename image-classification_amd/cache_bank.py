@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import operator
 
 import torch
 from torch import nn
@@ -40,17 +41,31 @@ def _on(device: torch.device):
     return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+_ARRAYS = {}                   # strides -> the same as a C array (there are few different ones; made anew they are 2 us a call)
+
+
 def _strides(t: torch.Tensor):
     """Strides of the sequence, head and row of a [batch, heads, rows, dim] tensor; a size of one has none."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    (a, b, c, _), (x, y, z, _) = t.shape, t.stride()
+    return (x if a > 1 else 0, y if b > 1 else 0, z if c > 1 else 0)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where its rows are contiguous and start on 16 bytes, else a copy that is so."""
-    step = 16 // t.element_size()
-    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and not any(s % step for s in _strides(t)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _array(strides):
+    known = _ARRAYS.get(strides)
+    if known is None:
+        if len(_ARRAYS) > 1024:
+            _ARRAYS.clear()
+        known = _ARRAYS[strides] = (ctypes.c_int64 * 3)(*strides)
+    return known
+
+
+def _aligned(t: torch.Tensor):
+    """``t`` itself where its rows are contiguous and start on 16 bytes, else a copy that is so; and its strides."""
+    step, strides = 16 // t.element_size(), _strides(t)
+    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and not (strides[0] % step or strides[1] % step or strides[2] % step):
+        return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _strides(t)
 
 
 class CacheBank(nn.Module):
@@ -62,7 +77,7 @@ class CacheBank(nn.Module):
         self.shapes = {}           # name -> (batch, heads, dim)
         self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows
         self._captured = set()     # names whose lengths a graph may change behind the host's back
-        self._views = {}           # name -> (buffers, mi_cache_t over them)
+        self._views = {}           # name -> (buffers, mi_cache_t over them, how to pick them)
 
     def __getstate__(self):
         return {**self.__dict__, "_views": {}}
@@ -91,10 +106,11 @@ class CacheBank(nn.Module):
     def _cache(self, name, what):
         if name not in self.sizes:
             raise KeyError(f"CacheBank.{what}: no bank named {name!r}")
-        held = tuple(self._buffers[f"{name}_{part}"] for part in _PARTS)
         known = self._views.get(name)
-        if known is not None and all(a is b for a, b in zip(known[0], held)):
-            return known[1], held
+        if known is not None and all(map(operator.is_, known[0], known[2](self._buffers))):
+            return known[1], known[0]
+        pick = operator.itemgetter(*[f"{name}_{part}" for part in _PARTS])
+        held = pick(self._buffers)
         if not held[0].is_cuda:
             raise RuntimeError(f"CacheBank.{what}: buffer is on {held[0].device}; image-classification_amd moves bank rows "
                                "with HIP kernels only (no CPU fallback) -- call .to(device) first")
@@ -103,8 +119,8 @@ class CacheBank(nn.Module):
                 raise RuntimeError(f"CacheBank.{what}: buffer {name}_{part} must be contiguous {dtype} on {held[0].device}, "
                                    f"got {t.dtype} on {t.device} (move banks with .to(device), not to another dtype)")
         batch, heads, dim = self.shapes[name]
-        view = _lib.Cache(*[t.data_ptr() for t in held], batch, heads, dim, held[4].shape[2], self.sizes[name])
-        self._views[name] = (held, view)
+        view = ctypes.pointer(_lib.Cache(*[t.data_ptr() for t in held], batch, heads, dim, held[4].shape[2], self.sizes[name]))
+        self._views[name] = (held, view, pick)
         return view, held
 
     @staticmethod
@@ -143,8 +159,11 @@ class CacheBank(nn.Module):
     def _set_bound(self, name, bound):
         self._bounds[name] = self.sizes[name] if name in self._captured else min(bound, self.sizes[name])
 
+    def _span(self, name) -> int:
+        """About how many rows are in use: what launches are sized by."""
+        return max(1, self.sizes[name] if name in self._captured else self._bounds[name])
+
     # --------------------------------------------------------------------------------------------------------------- calls
-    @torch.no_grad()
     def push(self, name, key, value, counts=None, held=False):
         """Appends ``key`` and ``value`` [batch, heads, T, dim] behind the last row of every sequence, quantised to 4 bits.
 
@@ -165,20 +184,22 @@ class CacheBank(nn.Module):
             if not self._changes(name):
                 bound = k if name in self._captured else self._bounds[name]
                 if bound + T > k:                       # the one place that waits for the device
-                    lengths = held_by[6]
-                    longest = int((lengths if counts is None else lengths + counts.clamp(0, T)).max()) + (T if counts is None else 0)
+                    longest = torch.empty(1, dtype=torch.int32, device=device)
+                    _lib.check(_lib.lib().mi_cache_longest(view, None if counts is None else counts.data_ptr(), T, longest.data_ptr(),
+                                                           _lib.raw_stream(device.index)), "mi_cache_longest")
+                    longest = int(longest)
                     if longest > k:
                         raise RuntimeError(f"CacheBank.push: {longest} rows do not fit bank {name!r} of {k}; evict or trim first")
-                    bound = longest - T if counts is None else longest
+                    bound = longest - T
                 self._set_bound(name, bound + T)
             else:
                 self._set_bound(name, k)
-            key, value = _aligned(key), _aligned(value)
+            (key, key_strides), (value, value_strides) = _aligned(key), _aligned(value)
             out = tuple(torch.empty(key.shape, dtype=key.dtype, device=device) for _ in range(2)) if held else (None, None)
-            _lib.check(_lib.lib().mi_cache_push(ctypes.byref(view), key.data_ptr(), (ctypes.c_int64 * 3)(*_strides(key)),
-                                                value.data_ptr(), (ctypes.c_int64 * 3)(*_strides(value)), _CODES[key.dtype], T,
+            _lib.check(_lib.lib().mi_cache_push(view, key.data_ptr(), _array(key_strides),
+                                                value.data_ptr(), _array(value_strides), _CODES[key.dtype], T,
                                                 None if counts is None else counts.data_ptr(), None if not held else out[0].data_ptr(),
-                                                None if not held else out[1].data_ptr(), _lib.stream_ptr(device)), "mi_cache_push")
+                                                None if not held else out[1].data_ptr(), _lib.raw_stream(device.index)), "mi_cache_push")
         return out if held else None
 
     def attend(self, name, query, counts=None, scale=None, causal=True, accumulate=False):
@@ -203,23 +224,24 @@ class CacheBank(nn.Module):
         counts = self._counts(counts, batch, T, device)
         L = _lib.lib()
         with _on(device):
-            query = _aligned(query)
+            query, query_strides = _aligned(query)
             out = torch.empty_like(query)
-            if out.stride(3) != 1 or any(s * out.element_size() % 16 for s in _strides(out)):
-                out = torch.empty(query.shape, dtype=query.dtype, device=device)
             if T == 0:
                 return out
-            span = max(1, self.sizes[name] if name in self._captured else self._bounds[name])
+            step, out_strides = 16 // out.element_size(), _strides(out)
+            if out.stride(3) != 1 or out_strides[0] % step or out_strides[1] % step or out_strides[2] % step:
+                out = torch.empty(query.shape, dtype=query.dtype, device=device)
+                out_strides = _strides(out)
+            span = self._span(name)
             code = _CODES[query.dtype]
-            nbytes = L.mi_cache_attend_workspace_bytes(ctypes.byref(view), code, T, group, span, int(causal), int(accumulate))
+            nbytes = L.mi_cache_attend_workspace_bytes(view, code, T, group, span, int(causal), int(accumulate))
             ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
-            _lib.check(L.mi_cache_attend(ctypes.byref(view), query.data_ptr(), (ctypes.c_int64 * 3)(*_strides(query)),
-                                         out.data_ptr(), (ctypes.c_int64 * 3)(*_strides(out)), code, T, group,
+            _lib.check(L.mi_cache_attend(view, query.data_ptr(), _array(query_strides),
+                                         out.data_ptr(), _array(out_strides), code, T, group,
                                          None if counts is None else counts.data_ptr(), scale, int(causal), int(accumulate), span,
-                                         ws.data_ptr(), ws.numel(), _lib.stream_ptr(device)), "mi_cache_attend")
+                                         ws.data_ptr(), ws.numel(), _lib.raw_stream(device.index)), "mi_cache_attend")
         return out
 
-    @torch.no_grad()
     def evict(self, name, keep, recent=0, into=None):
         """Cuts every head of every sequence down to ``keep`` rows: those among the last ``recent`` pushed of the sequence stay, then those
         with the largest :meth:`weights`, ties to the lower slot.  Slots below ``keep`` whose row leaves take, in ascending order, the kept
@@ -240,13 +262,12 @@ class CacheBank(nn.Module):
         L = _lib.lib()
         with _on(device):
             self._changes(target)
-            ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(ctypes.byref(view), keep)), dtype=torch.uint8, device=device)
-            span = max(1, self.sizes[name] if name in self._captured else self._bounds[name])
-            _lib.check(L.mi_cache_evict(ctypes.byref(view), ctypes.byref(other), keep, recent, span, ws.data_ptr(), ws.numel(),
-                                        _lib.stream_ptr(device)), "mi_cache_evict")
+            ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(view, keep)), dtype=torch.uint8, device=device)
+            span = self._span(name)
+            _lib.check(L.mi_cache_evict(view, other, keep, recent, span, ws.data_ptr(), ws.numel(),
+                                        _lib.raw_stream(device.index)), "mi_cache_evict")
         self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bounds[name]))
 
-    @torch.no_grad()
     def trim(self, name, lengths=0):
         """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
         the bank, a smaller length takes back the rows pushed last (a rejected draft).  Positions go on from the cut."""
@@ -263,11 +284,10 @@ class CacheBank(nn.Module):
             number = min(number, self.sizes[name])
         with _on(device):
             self._changes(name)
-            _lib.check(_lib.lib().mi_cache_trim(ctypes.byref(view), None if each is None else each.data_ptr(), number,
-                                                _lib.stream_ptr(device)), "mi_cache_trim")
+            _lib.check(_lib.lib().mi_cache_trim(view, None if each is None else each.data_ptr(), number,
+                                                _lib.raw_stream(device.index)), "mi_cache_trim")
         self._set_bound(name, self._bounds[name] if each is not None else min(number, self._bounds[name]))
 
-    @torch.no_grad()
     def __getitem__(self, name):
         """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""
         view, held_by = self._cache(name, "__getitem__")
@@ -275,7 +295,7 @@ class CacheBank(nn.Module):
         batch, heads, dim = self.shapes[name]
         with _on(device):
             out = tuple(torch.empty((batch, heads, self.sizes[name], dim), dtype=torch.bfloat16, device=device) for _ in range(2))
-            _lib.check(_lib.lib().mi_cache_read(ctypes.byref(view), out[0].data_ptr(), out[1].data_ptr(), _lib.stream_ptr(device)), "mi_cache_read")
+            _lib.check(_lib.lib().mi_cache_read(view, out[0].data_ptr(), out[1].data_ptr(), _lib.raw_stream(device.index)), "mi_cache_read")
         return out
 
     def lengths(self, name):

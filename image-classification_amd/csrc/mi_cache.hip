@@ -114,7 +114,7 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
         a.tiles = ceil_div(a.R, 32 * a.waves);
     } else {
         a.tiles = ceil_div(a.R, 16 * a.mt);
-        const int64_t ns = ceil_div(768, bh * a.tiles), most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
+        const int64_t ns = ceil_div(512, bh * a.tiles), most = std::min<int64_t>(ceil_div(span, 512), mi::CACHE_MAX_SPLIT);
         a.nsplit = ns > most ? most : ns;
     }
     const int64_t rows = c->batch * c->heads * a.R;
@@ -190,13 +190,24 @@ hipError_t launch_attend_w(int width, const mi::CacheAttendParams &p, const Atte
                                                                                          : launch_attend<DT, 8>(p, a, accumulate, s);
 }
 
+template <int DT, int W>
+void launch_push_w(const mi::PushParams &p, hipStream_t s)
+{
+    const int64_t lanes = (int64_t)p.c.heads * p.T * (W / 4);                    // of one sequence
+    if (lanes <= 2048) {
+        hipLaunchKernelGGL((mi::cache_push_kernel<DT, W, true>), dim3((unsigned)p.c.batch), dim3(256), 0, s, p);
+        return;
+    }
+    hipLaunchKernelGGL((mi::cache_push_kernel<DT, W, false>), dim3((unsigned)ceil_div(p.c.batch * lanes, 256)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(mi::cache_advance_kernel, dim3((unsigned)ceil_div(p.c.batch, 64)), dim3(64), 0, s, p);
+}
+
 template <int DT>
 void launch_push(int width, const mi::PushParams &p, hipStream_t s)
 {
-    const dim3 grid((unsigned)ceil_div((int64_t)p.c.batch * p.c.heads * p.T * (width / 4), 256));
-    if (width == 64) hipLaunchKernelGGL((mi::cache_push_kernel<DT, 64>), grid, dim3(256), 0, s, p);
-    else if (width == 128) hipLaunchKernelGGL((mi::cache_push_kernel<DT, 128>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((mi::cache_push_kernel<DT, 256>), grid, dim3(256), 0, s, p);
+    if (width == 64) launch_push_w<DT, 64>(p, s);
+    else if (width == 128) launch_push_w<DT, 128>(p, s);
+    else launch_push_w<DT, 256>(p, s);
 }
 
 bool known_dtype(int dtype) { return dtype == MI_F32 || dtype == MI_BF16 || dtype == MI_F16; }
@@ -231,7 +242,19 @@ int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_s
     else if (dtype == MI_BF16) launch_push<mi::CACHE_BF16>(width, p, s);
     else launch_push<mi::CACHE_F16>(width, p, s);
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(mi::cache_advance_kernel, dim3((unsigned)ceil_div(cache->batch, 64)), dim3(64), 0, s, p);
+    return MI_OK;
+}
+
+int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_longest"));
+    if (!out) return fail(MI_ERR_ARG, "mi_cache_longest: null pointer");
+    if (T < 0 || T > MAX_ROWS) return fail(MI_ERR_ARG, "mi_cache_longest: bad T=%lld", (long long)T);
+    mi::PushParams p{};
+    p.c = view(cache);
+    p.counts = counts;
+    p.T = (int)T;
+    hipLaunchKernelGGL(mi::cache_longest_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, p, out);
     HIP_CHECK(hipGetLastError());
     return MI_OK;
 }

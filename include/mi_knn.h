@@ -255,6 +255,9 @@ int64_t mi_cache_width(int64_t dim);
 int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_strides, const void *value, const int64_t *value_strides,
                   int dtype, int64_t T, const int32_t *counts, void *held_key, void *held_value, mi_stream_t stream);
 
+/* *out (device) = the most rows that a sequence would have after mi_cache_push of these counts, whether they fit or not. */
+int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream);
+
 /* length[b] = min(length[b], lengths[b]) (device int32[batch]; NULL: `length` for all); positions go on from the cut. */
 int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t length, mi_stream_t stream);
 

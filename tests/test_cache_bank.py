@@ -125,6 +125,7 @@ def test_abi_refuses_bad_calls_before_touching_the_device():
     assert push(held=(at, None)) == -1 and push(held=(at, at + 2)) == -1
     assert L.mi_cache_push(None, at, s, at, s, 1, 1, None, None, None, None) == -1
     assert L.mi_cache_trim(cache(), None, -1, None) == -1
+    assert L.mi_cache_longest(cache(), None, 1, None, None) == -1 and L.mi_cache_longest(cache(), None, -1, at, None) == -1
     assert L.mi_cache_read(cache(), None, at, None) == -1
 
     def attend(scale=1.0, ws=at, nbytes=1 << 30, group=1, T=1, dtype=1, out=at):
