@@ -161,15 +161,18 @@ template <int DT, int W, bool WHOLE>
 __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
 {
     constexpr int SIDE = W / 8, ROW = 2 * SIDE;
-    const int lane = threadIdx.x & 63;
-    const long long all = WHOLE ? (long long)p.c.heads * p.T : (long long)p.c.batch * p.c.heads * p.T;
-    for (long long at = (WHOLE ? 0 : (long long)blockIdx.x * 256) + threadIdx.x; at < (WHOLE ? (all * ROW + 255) / 256 * 256 : (long long)(blockIdx.x + 1) * 256); at += 256) {
-        const long long r = at / ROW;
-        const int c = (int)(at % SIDE), side = (int)(at / SIDE) & 1;
-        const bool in = r < all;
-        const long long rr = in ? r : 0;
-        const int t = (int)(rr % p.T), h = WHOLE ? (int)(rr / p.T) : (int)(rr / p.T % p.c.heads), b = WHOLE ? (int)blockIdx.x : (int)(rr / p.T / p.c.heads);
-        const int len = p.c.length[b], n = push_count(p, b, len);
+    constexpr int TURN = 256 / ROW, TURNS = 4;                   // rows a turn; turns of a workgroup that shares a sequence
+    const int lane = threadIdx.x & 63, c = threadIdx.x % SIDE, side = threadIdx.x / SIDE & 1;
+    // WHOLE: rows of all heads of sequence blockIdx.x; otherwise a stretch of one head's
+    const int chunks = WHOLE ? 1 : (p.T + TURN * TURNS - 1) / (TURN * TURNS);
+    const int group = (int)(blockIdx.x / chunks), b = WHOLE ? (int)blockIdx.x : group / p.c.heads;
+    const int first = WHOLE ? 0 : (int)(blockIdx.x % chunks) * TURN * TURNS, last = WHOLE ? p.c.heads * p.T : min(p.T, first + TURN * TURNS);
+    const int len = p.c.length[b], n = push_count(p, b, len);
+#pragma unroll WHOLE ? 1 : TURNS
+    for (int r0 = first; r0 < last; r0 += TURN) {
+        const int r = r0 + threadIdx.x / ROW;
+        const bool in = r < last;
+        const int h = WHOLE ? (in ? r / p.T : 0) : group - b * p.c.heads, t = WHOLE ? (in ? r - h * p.T : 0) : r;
         const bool real = in && t < n;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (real && c * 8 < p.c.dim) {
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
                 const float a = (low < 4 ? 0.5f * (float)low : low < 6 ? (float)(low - 2) : (float)(2 * low - 8)) * s;
                 v[i] = poison ? __uint_as_float(0x7fc00000u) : !real ? 0.f : four > 7 ? -a : a;
             }
-            const long long at_row = WHOLE ? (long long)b * all + r : r;
+            const long long at_row = ((long long)b * p.c.heads + h) * p.T + t;
             store8<DT>(held + (at_row * p.c.dim + c * 8) * elem_bytes<DT>(), v);
         }
     }
@@ -275,30 +278,50 @@ __global__ void cache_trim_kernel(CacheView c, const int *lengths, int length)
     }
 }
 
-// ---------------------------------------------------------------------------------------------------------- read back
-// Rows [0, limit) of every sequence and head as bf16 (exact); rows behind the last one are zeros.  A lane takes 8 dims.
-template <int W>
-__global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, uint4 *key, uint4 *value)
+// ------------------------------------------------------------------------------------------------ 4 bits to bf16
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ float scale_of(uint32_t word, int e) { return __uint_as_float(((word >> (8 * e)) & 255u) << 23); }
+
+template <int I>
+__device__ __forceinline__ uint32_t cvt2(uint32_t w, float s)
 {
-    constexpr int SIDE = W / 8, ROW = 2 * SIDE;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long r = at / ROW;
-    const int d = (int)(at % SIDE), side = (int)(at / SIDE) & 1;
-    if (r >= (long long)c.batch * c.heads * c.limit || d * 8 >= c.dim) return;
-    const long long bh = r / c.limit, slot = r % c.limit;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (slot < c.length[bh / c.heads]) {
-        const uint32_t code = *(const uint32_t *)((side ? c.value : c.key) + (bh * c.rows + slot) * (W / 2) + d * 4);
-        const uint32_t byte = (side ? c.value_scale : c.key_scale)[(bh * (W / 32) + d / 4) * c.rows + slot];
-        const float s = __uint_as_float(byte << 23);
-        v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0));
-        v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1));
-        v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2));
-        v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3));
-        const bool nan = (side ? c.key_scale[(bh * (W / 32) + d / 4) * c.rows + slot] : byte) == 255;
-        if (nan) v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+}
+
+__device__ __forceinline__ cb16x8 cvt8(uint32_t w, float s)
+{
+    const uint4 v = make_uint4(cvt2<0>(w, s), cvt2<1>(w, s), cvt2<2>(w, s), cvt2<3>(w, s));
+    return __builtin_bit_cast(cb16x8, v);
+}
+
+// ---------------------------------------------------------------------------------------------------------- read back
+// Rows [0, limit) of every sequence and head as bf16 (exact); rows behind the last one are zeros.  A lane takes 8 dims of a row; a
+// workgroup CACHE_READ_TURNS * 2048 / W rows of one head, so that nothing is divided by (with a row found by 64-bit divisions: 93 us for
+// 2064 rows of 256 heads, 128 wide).
+constexpr int CACHE_READ_TURNS = 8;
+
+template <int W>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, uint4 *key, uint4 *value, int chunks)
+{
+    constexpr int SIDE = W / 8, ROW = 2 * SIDE, TURN = 256 / ROW;
+    const long long bh = blockIdx.x / chunks;
+    const int d = threadIdx.x % SIDE, side = threadIdx.x / SIDE & 1, first = (int)(blockIdx.x % chunks) * TURN * CACHE_READ_TURNS;
+    if (d * 8 >= c.dim) return;
+    const int len = c.length[bh / c.heads];
+    const uint8_t *codes = (side ? c.value : c.key) + bh * c.rows * (W / 2) + d * 4;
+    const uint8_t *scales = (side ? c.value_scale : c.key_scale) + (bh * (W / 32) + d / 4) * c.rows, *nans = c.key_scale + (bh * (W / 32) + d / 4) * c.rows;
+    uint4 *out = (side ? value : key) + bh * c.limit * (c.dim / 8) + d;
+#pragma unroll
+    for (int turn = 0; turn < CACHE_READ_TURNS; ++turn) {
+        const int slot = first + turn * TURN + threadIdx.x / ROW;
+        if (slot >= c.limit) continue;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (slot < len) {
+            v = __builtin_bit_cast(uint4, cvt8(*(const uint32_t *)(codes + (long long)slot * (W / 2)), scale_of(scales[slot])));
+            if (nans[slot] == 255) v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        }
+        out[(long long)slot * (c.dim / 8)] = v;
     }
-    (side ? value : key)[r * (c.dim / 8) + d] = v;
 }
 
 // ---------------------------------------------------------------------------------------------------------- attention
@@ -356,21 +379,6 @@ __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[
 }
 
 template <int DT> struct Pieces { static constexpr int N = DT == CACHE_F32 ? 3 : DT == CACHE_F16 ? 2 : 1; };
-
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-__device__ __forceinline__ float scale_of(uint32_t word, int e) { return __uint_as_float(((word >> (8 * e)) & 255u) << 23); }
-
-template <int I>
-__device__ __forceinline__ uint32_t cvt2(uint32_t w, float s)
-{
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
-}
-
-__device__ __forceinline__ cb16x8 cvt8(uint32_t w, float s)
-{
-    const uint4 v = make_uint4(cvt2<0>(w, s), cvt2<1>(w, s), cvt2<2>(w, s), cvt2<3>(w, s));
-    return __builtin_bit_cast(cb16x8, v);
-}
 
 // NB words of 8 elements / NB bytes of 2 elements at p, as words (one load each).
 template <int NB>
@@ -1360,18 +1368,23 @@ __device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, 
         const uint32_t mask = pass == 2 ? 1023u : 2047u;
         for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) s_hist[i] = 0;
         __syncthreads();
-        for (int i0 = wave * 64; i0 < n; i0 += EVICT_THREADS) {
-            const int i = i0 + lane;
-            const uint32_t r = i < n ? rank(i) : 0u;
-            const bool in = i < n && (r & known) == prefix;
-            const int digit = (int)((r >> shift) & mask);
-            // equal neighbours (rows that nothing attended to yet) are counted once for the wave, not 64 times in turn
-            const unsigned long long who = __ballot(in);
-            if (!who) continue;
-            const int first = __builtin_amdgcn_readlane(digit, __ffsll((long long)who) - 1);
-            const unsigned long long same = __ballot(in && digit == first);
-            if (lane == 0) atomicAdd(&s_hist[first], __popcll(same));
-            if (in && digit != first) atomicAdd(&s_hist[digit], 1);
+        for (int i0 = wave * 64; i0 < n; i0 += 4 * EVICT_THREADS) {
+            uint32_t r[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[k] = i0 + k * EVICT_THREADS + lane < n ? rank(i0 + k * EVICT_THREADS + lane) : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = i0 + k * EVICT_THREADS + lane < n && (r[k] & known) == prefix;
+                const int digit = (int)((r[k] >> shift) & mask);
+                // equal neighbours (rows that nothing attended to yet) are counted once for the wave, not 64 times in turn
+                const unsigned long long who = __ballot(in);
+                if (who) {
+                    const int first = __builtin_amdgcn_readlane(digit, __ffsll((long long)who) - 1);
+                    const unsigned long long same = __ballot(in && digit == first);
+                    if (lane == 0) atomicAdd(&s_hist[first], __popcll(same));
+                    if (in && digit != first) atomicAdd(&s_hist[digit], 1);
+                }
+            }
         }
         __syncthreads();
         // the bin that holds the left-th largest: bins from the top, two a thread
@@ -1389,6 +1402,7 @@ __device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, 
             const bool second = above + a < left;
             s_pick[0] = second ? top - 1 : top;
             s_pick[1] = left - above - (second ? a : 0);
+            s_pick[2] = second ? b : a;                           // rows in it
         }
         __syncthreads();
         prefix |= (uint32_t)s_pick[0] << shift;
@@ -1400,31 +1414,44 @@ __device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, 
     const uint32_t edge = prefix;
     const int seg = ((n + EVICT_THREADS - 1) / EVICT_THREADS) * 64, lo = min(n, wave * seg), hi = min(n, lo + seg);
     const unsigned long long below = (1ull << lane) - 1;
-    int eq = 0;
-    for (int i0 = lo; i0 < hi; i0 += 64) eq += __popcll(__ballot(i0 + lane < hi && rank(i0 + lane) == edge));
+    const bool all_ties = s_pick[2] == left;                      // the usual case: every row on the edge stays
     int2 all;
-    const int eq0 = wave_scan2(make_int2(eq, 0), s_wave, all).x;
+    int eq0 = 0;
+    if (!all_ties) {
+        int eq = 0;
+        for (int i0 = lo; i0 < hi; i0 += 64) eq += __popcll(__ballot(i0 + lane < hi && rank(i0 + lane) == edge));
+        eq0 = wave_scan2(make_int2(eq, 0), s_wave, all).x;
+    }
     int2 off = make_int2(0, 0);              // freed slots below keep, kept rows from there on
     int base = 0;                            // pairs before those of the freed slots
 #pragma unroll
     for (int write = 0; write < 2; ++write) {
         int at = eq0, holes = 0, tails = 0;
-        for (int i0 = lo; i0 < hi; i0 += 64) {
-            const int i = i0 + lane;
-            const uint32_t r = i < hi ? rank(i) : 0u;
-            const unsigned long long on = __ballot(i < hi && r == edge);
-            const bool kept = i < hi && (r > edge || (r == edge && at + __popcll(on & below) < left));
-            const bool hole = i < hi && i < keep && !kept, tail = i >= keep && kept;
-            const unsigned long long h = __ballot(hole), t = __ballot(tail);
-            if (write) {
-                const int nh = off.x + holes + __popcll(h & below), nt = off.y + tails + __popcll(t & below);
-                if (hole) pairs[base + nh].x = i;
-                if (tail) pairs[base + nt].y = i;
-                if (base && i < keep && kept) pairs[i - nh] = make_int2(i, i);
+        for (int i1 = lo; i1 < hi; i1 += 256) {
+            uint32_t rs[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) rs[k] = i1 + 64 * k + lane < hi ? rank(i1 + 64 * k + lane) : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i1 + 64 * k + lane;
+                const uint32_t r = rs[k];
+                bool kept = i < hi && r >= edge;
+                if (!all_ties) {
+                    const unsigned long long on = __ballot(i < hi && r == edge);
+                    kept = i < hi && (r > edge || (r == edge && at + __popcll(on & below) < left));
+                    at += __popcll(on);
+                }
+                const bool hole = i < hi && i < keep && !kept, tail = i >= keep && kept;
+                const unsigned long long h = __ballot(hole), t = __ballot(tail);
+                if (write) {
+                    const int nh = off.x + holes + __popcll(h & below), nt = off.y + tails + __popcll(t & below);
+                    if (hole) pairs[base + nh].x = i;
+                    if (tail) pairs[base + nt].y = i;
+                    if (base && i < keep && kept) pairs[i - nh] = make_int2(i, i);
+                }
+                holes += __popcll(h);
+                tails += __popcll(t);
             }
-            at += __popcll(on);
-            holes += __popcll(h);
-            tails += __popcll(t);
         }
         if (!write) {
             off = wave_scan2(make_int2(holes, tails), s_wave, all);
@@ -1442,7 +1469,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams
     extern __shared__ uint32_t s_rank[];
     __shared__ int s_hist[EVICT_BINS];
     __shared__ int2 s_wave[EVICT_THREADS / 64];
-    __shared__ int s_pick[2];
+    __shared__ int s_pick[3];
     const long long bh = blockIdx.x;
     const int b = (int)(bh / p.c.heads), tid = threadIdx.x;
     int n = p.c.length[b];
@@ -1457,6 +1484,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams
     const float *w = p.c.weight + bh * p.c.rows;
     const int *pos = p.c.position + bh * p.c.rows;
     if (n <= resident) {
+#pragma unroll 4
         for (int i = tid * 4; i < n; i += EVICT_THREADS * 4) {        // rows are allocated in 64s: whole vectors
             const float4 x = *(const float4 *)(w + i);
             const int4 y = *(const int4 *)(pos + i);

@@ -198,7 +198,8 @@ void launch_push_w(const mi::PushParams &p, hipStream_t s)
         hipLaunchKernelGGL((mi::cache_push_kernel<DT, W, true>), dim3((unsigned)p.c.batch), dim3(256), 0, s, p);
         return;
     }
-    hipLaunchKernelGGL((mi::cache_push_kernel<DT, W, false>), dim3((unsigned)ceil_div(p.c.batch * lanes, 256)), dim3(256), 0, s, p);
+    const int64_t stretches = ceil_div(p.T, 1024 / (W / 4));                     // as the kernel cuts a head's rows
+    hipLaunchKernelGGL((mi::cache_push_kernel<DT, W, false>), dim3((unsigned)((int64_t)p.c.batch * p.c.heads * stretches)), dim3(256), 0, s, p);
     hipLaunchKernelGGL(mi::cache_advance_kernel, dim3((unsigned)ceil_div(p.c.batch, 64)), dim3(64), 0, s, p);
 }
 
@@ -273,14 +274,14 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
     MI_TRY(check_cache(cache, "mi_cache_read"));
     if (!key || !value || (((uintptr_t)key | (uintptr_t)value) & 15)) return fail(MI_ERR_ARG, "mi_cache_read: key and value must be 16-byte aligned");
     const int width = width_of(cache->dim);
-    const int64_t blocks = ceil_div(cache->batch * cache->heads * cache->limit * (width / 4), 256);
+    const int64_t chunks = ceil_div(cache->limit, mi::CACHE_READ_TURNS * (1024 / width)), blocks = cache->batch * cache->heads * chunks;
     MI_TRY(check_grid("mi_cache_read", blocks));
     const dim3 grid((unsigned)blocks);
     hipStream_t s = (hipStream_t)stream;
     const mi::CacheView v = view(cache);
-    if (width == 64) hipLaunchKernelGGL(mi::cache_read_kernel<64>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
-    else if (width == 128) hipLaunchKernelGGL(mi::cache_read_kernel<128>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
-    else hipLaunchKernelGGL(mi::cache_read_kernel<256>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value);
+    if (width == 64) hipLaunchKernelGGL(mi::cache_read_kernel<64>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value, (int)chunks);
+    else if (width == 128) hipLaunchKernelGGL(mi::cache_read_kernel<128>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value, (int)chunks);
+    else hipLaunchKernelGGL(mi::cache_read_kernel<256>, grid, dim3(256), 0, s, v, (uint4 *)key, (uint4 *)value, (int)chunks);
     HIP_CHECK(hipGetLastError());
     return MI_OK;
 }
