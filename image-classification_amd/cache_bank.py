@@ -6,7 +6,6 @@ the keys and values of an attention layer do; ``heads=1, batch=1`` is a plain fe
 
     bank = CacheBank()
     bank.register("layer0", dim=128, k=4096, heads=8, batch=64)
-    bank = bank.cuda()
     bank.push("layer0", key, value)                            # [batch, heads, T, dim], quantised to 4.25 bits a value
     out = bank.attend("layer0", query, accumulate=True)        # [batch, heads * group, T, dim]; also sums what each row got
     bank.evict("layer0", keep=2048, recent=256)                # the least attended rows leave
@@ -87,7 +86,10 @@ class CacheBank(nn.Module):
         self._bounds = dict(self.sizes)
 
     def register(self, name, dim, k, heads=1, batch=1, device=None):
-        """An empty bank of ``k`` rows of ``dim`` values (a multiple of 8, at most 256) for each head of each sequence."""
+        """An empty bank of ``k`` rows of ``dim`` values (a multiple of 8, at most 256) for each head of each sequence, on ``device``
+        (the current HIP device where there is one: such banks are large, and of no use elsewhere)."""
+        if device is None and torch.cuda.is_available():
+            device = torch.device("cuda", torch.cuda.current_device())
         dim, k, heads, batch = int(dim), int(k), int(heads), int(batch)
         if dim < 8 or dim > 256 or dim % 8:
             raise ValueError(f"dim must be a multiple of 8 in [8, 256], got {dim}")

@@ -341,7 +341,9 @@ struct CacheAttendParams {
     int chunks;                              // weights: workgroups along the bank's rows of a (sequence, head); each takes every chunks-th stretch
     int rsplit;                              // weights, many query rows: pieces of the query rows ...
     float *part_w;                           //          ... and their sums, [piece][batch heads][rows]
-    float *lse;                              // [batch heads][R] log2 of the softmax denominator (weights wanted), or null
+    float2 *norm;                            // [batch heads][R] what turns a score into a probability (weights wanted), or null:
+                                             // p = exp2(s c2 - x) y.  (As one number, the log of the denominator, it would
+                                             // cost a rounding of 2^-19 of each p where scores are 16 to 32.)
     float *scores;                           // [batch heads][R][rows] scores before the scale (few query rows, weights wanted), or null
 };
 
@@ -694,7 +696,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 for (int i = 0; i < 8; ++i) x[i] = den == 0.f ? 0.f : x[i] * inv;
                 const int t = row / p.G, g = row - t * p.G;
                 if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-                if (p.lse && d == 0) p.lse[bh * p.R + row] = den == 0.f ? INFINITY : rref + __builtin_amdgcn_logf(den);
+                if (p.norm && d == 0) p.norm[bh * p.R + row] = make_float2(rref, den == 0.f ? 0.f : inv);
             }
         }
     }
@@ -963,7 +965,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
         for (int i = 0; i < NB; ++i) x[i] = none ? 0.f : o[i][r] * inv;
         store_n<DT, NB>(to + (long long)d * elem_bytes<DT>(), x);
     }
-    if (p.lse && l == 0) p.lse[bh * p.R + row] = none ? INFINITY : (ref == -INFINITY ? 0.f : ref) + __builtin_amdgcn_logf(sum);
+    if (p.norm && l == 0) p.norm[bh * p.R + row] = make_float2(ref == -INFINITY ? 0.f : ref, none ? 0.f : inv);
 }
 
 // Joins the pieces of a row: W / 8 lanes side by side in a piece.  More than 8 pieces: one workgroup a row, 2048 / W pieces at a time
@@ -980,7 +982,7 @@ __device__ __forceinline__ void store_joined(const CacheAttendParams &p, long lo
     const long long bh = g0 / p.R;
     const int row = (int)(g0 % p.R), b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads), t = row / p.G, g = row - t * p.G;
     if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-    if (p.lse && d == 0) p.lse[g0] = big == -INFINITY ? INFINITY : big + __builtin_amdgcn_logf(den);
+    if (p.norm && d == 0) p.norm[g0] = big == -INFINITY ? make_float2(0.f, 0.f) : make_float2(big, inv);
 }
 
 template <int DT, int W>
@@ -1059,7 +1061,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p)
     store_joined<DT, W>(p, g0, d, x, big, den);
 }
 
-// Attention sums: weight[slot] += sum over the query rows of exp(s - lse).  A wave has one unit of 32 bank rows and goes over
+// Attention sums: weight[slot] += sum over the query rows of their probabilities.  A wave has one unit of 32 bank rows and goes over
 // all rows that may see it, so that every sum has one owner and one order.
 template <int DT, int NB>
 __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
@@ -1084,7 +1086,7 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
             const int lim = in ? visible(row / p.G, n, len, p.causal) : 0;
             cb16x8 q[NB][PQ];
             load_query<DT, NB, PQ>(p, b, h, in ? row : 0, j, lim > 0, q);
-            const float lse = lim > 0 ? p.lse[bh * p.R + row] : INFINITY;
+            const float2 norm = lim > 0 ? p.norm[bh * p.R + row] : make_float2(0.f, 0.f);
             cf32x4 s[2] = {cf32x4{0, 0, 0, 0}, cf32x4{0, 0, 0, 0}};
 #pragma unroll
             for (int a = 0; a < 2; ++a)
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
                 }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], p.c2, -lse));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], p.c2, -norm.x)) * norm.y;
                 w[e] += u0 + 16 * (e >> 2) + 4 * j + (e & 3) < lim ? x : 0.f;
             }
         }
@@ -1152,7 +1154,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
 #pragma unroll
         for (int r = 0; r < 16; ++r) w[r] = 0.f;
         // tiles before the first row that sees slot w0 are left out; those before the first that sees all slots of the workgroup
-        // are masked (rows that are not real divide by infinity)
+        // are masked (rows that are not real count zero times)
         const int t_lo = p.causal ? max(0, w0 - (len - n)) : 0, t_all = p.causal ? max(0, w0 + 255 - (len - n)) : 0;
         const int first = max(piece * per, (int)min((long long)tiles, (long long)t_lo * p.G / QROWS)), last = min(tiles, (piece + 1) * per);
         const int border = max(first, (int)min((long long)last, ((long long)t_all * p.G + QROWS - 1) / QROWS));
@@ -1164,15 +1166,15 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
                 g[a] = first * QROWS + 32 * a + c - t[a] * p.G;
             }
             uint4 mine[MINE * PQ];
-            float off[3][RT];                                     // less the log2 of the denominator: of the tile in hand, the next, the one loaded
+            float2 norm[3][RT];                                   // of the tile in hand, the next, the one loaded
             int see[3][RT];
             const auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int a = 0; a < RT; ++a) {
                     const bool real = t[a] < n;
                     see[2][a] = real ? visible(t[a], n, len, p.causal) : 0;
-                    const float lse = p.lse[bh * p.R + (real ? t[a] * p.G + g[a] : 0)];
-                    off[2][a] = see[2][a] > 0 ? -lse : -INFINITY;
+                    const float2 row = p.norm[bh * p.R + (real ? t[a] * p.G + g[a] : 0)];
+                    norm[2][a] = make_float2(real ? -row.x : 0.f, real ? row.y : 0.f);
                 }
 #pragma unroll
                 for (int m = 0; m < MINE; ++m) {
@@ -1204,7 +1206,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
 #pragma unroll
                 for (int m = 0; m < MINE * PQ; ++m) s_q[(tile - first) & 1][wave * MINE * PQ + m][lane] = mine[m];
 #pragma unroll
-                for (int a = 0; a < RT; ++a) off[0][a] = off[1][a], off[1][a] = off[2][a], see[0][a] = see[1][a], see[1][a] = see[2][a];
+                for (int a = 0; a < RT; ++a) norm[0][a] = norm[1][a], norm[1][a] = norm[2][a], see[0][a] = see[1][a], see[1][a] = see[2][a];
             };
             const auto product = [&](int tile, cf32x16 (&s)[RT]) __attribute__((always_inline)) {
 #pragma unroll
@@ -1226,9 +1228,9 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
                 for (int a = 0; a < RT; ++a)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, off[0][a]));
-                        if constexpr (decltype(masked)::value) w[r] += u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[0][a] ? x : 0.f;
-                        else w[r] += x;
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, norm[0][a].x)), more = fmaf(x, norm[0][a].y, w[r]);
+                        if constexpr (decltype(masked)::value) w[r] = u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[0][a] ? more : w[r];
+                        else w[r] = more;
                     }
                 leave(tile);                                      // tile + 2, into the buffer that this tile had
                 fetch();
@@ -1301,11 +1303,11 @@ __global__ __launch_bounds__(256) void cache_weigh_scores_kernel(CacheAttendPara
         for (int row = 0; row < p.R; ++row) {
             const int lim = visible(row / p.G, n, len, p.causal);
             if (lim <= slot) continue;                    // (scores of a unit that no row of the tile sees were never written)
-            const float lse = p.lse[bh * p.R + row];
+            const float2 norm = p.norm[bh * p.R + row];
             const cf32x4 s = *(const cf32x4 *)(p.scores + (bh * p.R + row) * p.c.rows + slot);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[e], p.c2, -lse));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[e], p.c2, -norm.x)) * norm.y;
                 w[e] += slot + e < lim ? x : 0.f;
             }
         }

@@ -75,7 +75,7 @@ struct AttendPlan {
     int waves;
     int64_t chunks, rsplit;                  // weights: workgroups a (sequence, head) along the bank, and along the query rows
     bool scores;                             // weights: from scores left behind, not from a second product
-    size_t off_ml, off_lse, off_scores, off_w, total;
+    size_t off_ml, off_norm, off_scores, off_w, total;
 };
 
 // How long the tiled form takes, in tiles of 128 rows of the bank by 256 query rows on one compute unit, with `waves` waves a
@@ -124,8 +124,8 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
         a.off_ml = at;
         at += (size_t)round_up(a.nsplit * rows * 8, 256);
     }
-    a.off_lse = at;
-    if (accumulate) at += (size_t)round_up(rows * 4, 256);
+    a.off_norm = at;
+    if (accumulate) at += (size_t)round_up(rows * 8, 256);
     // A slot's attention sum costs 8 R bytes if its scores are written and read again, or its key, W / 2 + W / 32 bytes, and the
     // product once more.  Scores are laid out by the capacity (a captured call may see longer sequences than `span`).
     const int64_t score_bytes = rows * c->rows * 4;
@@ -324,7 +324,7 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     p.rsplit = (int)a.rsplit;
     p.part_w = (float *)((char *)workspace + a.off_w);
     p.scores = a.scores ? (float *)((char *)workspace + a.off_scores) : nullptr;
-    p.lse = accumulate ? (float *)((char *)workspace + a.off_lse) : nullptr;
+    p.norm = accumulate ? (float2 *)((char *)workspace + a.off_norm) : nullptr;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == MI_F32) HIP_CHECK(launch_attend_w<mi::CACHE_F32>(width, p, a, accumulate, s));
     else if (dtype == MI_BF16) HIP_CHECK(launch_attend_w<mi::CACHE_BF16>(width, p, a, accumulate, s));

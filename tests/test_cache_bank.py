@@ -23,7 +23,7 @@ def _ica():
 
 def _bank(batch, heads, dim, k, name="kv"):
     bank = _ica().CacheBank()
-    bank.register(name, dim=dim, k=k, heads=heads, batch=batch)
+    bank.register(name, dim=dim, k=k, heads=heads, batch=batch, device="cpu")
     return bank.cuda()
 
 
@@ -86,7 +86,7 @@ def test_refusals_on_the_cpu():
     for bad in (dict(k=0), dict(k=8, heads=0), dict(k=8, batch=0)):
         with pytest.raises(ValueError, match="positive"):
             bank.register("x", dim=64, **bad)
-    bank.register("kv", dim=64, k=100, heads=2, batch=3)
+    bank.register("kv", dim=64, k=100, heads=2, batch=3, device="cpu")
     assert bank.sizes["kv"] == 100 and set(bank.state_dict()) == {f"kv_{p}" for p in
                                                                   ("key", "key_scale", "value", "value_scale", "weight", "position", "length", "seen")}
     assert bank._buffers["kv_key"].shape == (3, 2, 128, 32)
@@ -594,6 +594,8 @@ def test_other_streams_state_dicts_and_copies():
     z = torch.zeros(2, 1, 20, 64, device="cuda")
     with pytest.raises(RuntimeError, match="do not fit"):                               # lengths came with the state
         twin.push("kv", z, z)
+    bank.register("here", dim=64, k=4, batch=2)
+    assert bank.lengths("here").is_cuda
     other = copy.deepcopy(bank)
     other.trim("kv")
     assert torch.equal(bank.attend("kv", q), want) and not other.attend("kv", q).any()
