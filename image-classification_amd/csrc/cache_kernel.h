@@ -493,6 +493,20 @@ __device__ __forceinline__ float across_j_sum(float x)
     return x + __shfl_xor(x, 32);
 }
 
+// A running sum of probabilities with what its roundings lost beside it: added one by one to the sum of a row that one slot dominates,
+// thousands of small ones would vanish (attention sums 3e-6 off for a row on 16 k slots).
+struct LongSum {
+    float sum = 0.f, lost = 0.f;
+    __device__ __forceinline__ void add(float x)
+    {
+        const float t = sum + x;
+        lost += fabsf(sum) >= fabsf(x) ? (sum - t) + x : (x - t) + sum;
+        sum = t;
+    }
+    __device__ __forceinline__ void scale(float f) { sum *= f, lost *= f; }
+    __device__ __forceinline__ float value() const { return sum + lost; }
+};
+
 // Streaming form: a workgroup has MT tiles of 16 query rows of one (sequence, head) and one piece of its bank rows; its four
 // waves take every fourth unit of 32 rows each, straight from memory into registers, and are joined at the end.
 template <int DT, int NB, int MT>
@@ -550,12 +564,12 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
     const int first = split * per, last = min(units, first + per);
 
     cf32x4 o[MT][2 * NB];
-    float mx[MT], ref[MT], sum[MT];          // maximum, its share of the exponent, sum of this lane's probabilities
+    float mx[MT], ref[MT];                   // maximum, its share of the exponent
+    LongSum sum[MT];                         // of this lane's probabilities
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         mx[m] = -INFINITY;
         ref[m] = 0.f;
-        sum[m] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) o[m][i] = cf32x4{0, 0, 0, 0};
     }
@@ -604,16 +618,17 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 ref[m] = now == -INFINITY ? 0.f : now * p.c2;
                 const float shrink = __builtin_amdgcn_exp2f(fmaf(mx[m], p.c2, -ref[m]));
                 mx[m] = now;
-                sum[m] *= shrink;
+                sum[m].scale(shrink);
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[m][i] *= shrink;
             }
-            float x[8];
+            float x[8], part = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], p.c2, -ref[m]));
-                sum[m] += x[e];
+                part += x[e];
             }
+            sum[m].add(part);
             split_pieces<PP, false>(x, pf[m]);
         }
 #pragma unroll
@@ -659,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
     // join the four waves, one tile of 16 rows at a time (what the loop read of shared memory is read: the barrier below)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        const float l = across_j_sum(sum[m]);
+        const float l = across_j_sum(sum[m].value());
         __syncthreads();
         if (j == 0) {
             s_m[wave][c] = mx[m];
@@ -832,7 +847,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-    float ref = -INFINITY, sum = 0.f, top = -INFINITY;            // reference of the exponent (log2 units), sum, largest score of a tile
+    float ref = -INFINITY, top = -INFINITY;                       // reference of the exponent (log2 units), largest score of a tile
+    LongSum total;
 
     if (first < last) {
         const TileAt<NB> at(p.c, bh, lane, wave & 3);
@@ -873,13 +889,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
             const float now = fmaxf(ref, fmaxf(top, __shfl_xor(top, 32)) * p.c2);
             const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - now);
             ref = now;
-            sum *= shrink;
+            total.scale(shrink);
 #pragma unroll
             for (int i = 0; i < NB; ++i) o[i] *= shrink;
         };
         const auto apply = [&](int un) __attribute__((always_inline)) {
             const uint4 *values = s_tile + ((un - first) & 1) * (KF + VF) * 64 + KF * 64;
             const float off = ref == -INFINITY ? 0.f : -ref;
+            float sum = 0.f;
 #pragma unroll
             for (int sq = 0; sq < 2 * SUB; ++sq) {
                 float x[8];
@@ -901,6 +918,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
                     for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[i], 0, 0, 0);
                 }
             }
+            total.add(sum);
         };
         load(first);
         leave(first);
@@ -937,6 +955,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
         }
         apply(un);
     }
+    float sum = total.value();
     sum += __shfl_xor(sum, 32);
     if (row >= p.R) return;
     const bool none = !real || sum == 0.f;                        // (a row that sees nothing but NaN is NaN)
