@@ -580,11 +580,11 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
         else return q[m][i][k];
     };
     const auto compute = [&](int u0, const Unit<NB> &u) __attribute__((always_inline)) {
-        cf32x4 s[MT][2];
+        cf32x4 s[MT][2], small[PQ > 1 ? MT : 1][2];               // products of the query's first piece, and of the others
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) s[m][a] = cf32x4{0, 0, 0, 0};
+            for (int m = 0; m < MT; ++m) s[m][a] = small[PQ > 1 ? m : 0][a] = cf32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const cb16x8 kf[2] = {key_operand<NB>(u.k[0], u.ks[0], i), key_operand<NB>(u.k[1], u.ks[1], i)};
@@ -594,9 +594,18 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 for (int k = 0; k < PQ; ++k) {
                     const cb16x8 qf = query(m, i, k);
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) s[m][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], qf, s[m][a], 0, 0, 0);
+                    for (int a = 0; a < 2; ++a) {
+                        cf32x4 &to = k ? small[PQ > 1 ? m : 0][a] : s[m][a];
+                        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], qf, to, 0, 0, 0);
+                    }
                 }
             if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (PQ > 1) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) s[m][a] += small[m][a];
         }
         cb16x8 pf[MT][PP];
 #pragma unroll
@@ -862,18 +871,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
         // scores of a tile and the largest of them
         const auto product = [&](int un, auto masked) __attribute__((always_inline)) {
             const uint4 *keys = s_tile + ((un - first) & 1) * (KF + VF) * 64;
+            cf32x16 small[PQ > 1 ? SUB : 1];                      // products of the query's smaller pieces
 #pragma unroll
             for (int tt = 0; tt < SUB; ++tt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[tt][r] = 0.f;
+                for (int r = 0; r < 16; ++r) s[tt][r] = small[PQ > 1 ? tt : 0][r] = 0.f;
 #pragma unroll
             for (int i = 0; i < SK; ++i)
 #pragma unroll
                 for (int tt = 0; tt < SUB; ++tt) {
                     const cb16x8 kf = __builtin_bit_cast(cb16x8, keys[(tt * SK + i) * 64 + lane]);
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k) s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], s[tt], 0, 0, 0);
+                    for (int k = 0; k < PQ; ++k) {
+                        cf32x16 &to = k ? small[PQ > 1 ? tt : 0] : s[tt];
+                        to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], to, 0, 0, 0);
+                    }
                 }
+            if constexpr (PQ > 1) {
+#pragma unroll
+                for (int tt = 0; tt < SUB; ++tt) s[tt] += small[tt];
+            }
             if constexpr (decltype(masked)::value) {
                 const int left = lim - un * TOKENS - 4 * l;
 #pragma unroll
@@ -1106,15 +1123,20 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
             cb16x8 q[NB][PQ];
             load_query<DT, NB, PQ>(p, b, h, in ? row : 0, j, lim > 0, q);
             const float2 norm = lim > 0 ? p.norm[bh * p.R + row] : make_float2(0.f, 0.f);
-            cf32x4 s[2] = {cf32x4{0, 0, 0, 0}, cf32x4{0, 0, 0, 0}};
+            cf32x4 s[2] = {cf32x4{0, 0, 0, 0}, cf32x4{0, 0, 0, 0}}, small[2] = {cf32x4{0, 0, 0, 0}, cf32x4{0, 0, 0, 0}};
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int a = 0; a < 2; ++a) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     const cb16x8 kf = key_operand<NB>(kk[a], ks[a], i);
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k) s[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i][k], s[a], 0, 0, 0);
+                    for (int k = 0; k < PQ; ++k) {
+                        cf32x4 &to = k ? small[a] : s[a];
+                        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i][k], to, 0, 0, 0);
+                    }
                 }
+                if constexpr (PQ > 1) s[a] += small[a];
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], p.c2, -norm.x)) * norm.y;
@@ -1232,10 +1254,11 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
                 for (int a = 0; a < RT; ++a)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
+                // the smaller pieces first
 #pragma unroll
-                for (int i = 0; i < SK; ++i)
+                for (int k = PQ - 1; k >= 0; --k)
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k)
+                    for (int i = 0; i < SK; ++i)
 #pragma unroll
                         for (int a = 0; a < RT; ++a)
                             s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], __builtin_bit_cast(cb16x8, s_q[(tile - first) & 1][(a * SK + i) * PQ + k][lane]), s[a], 0, 0, 0);
