@@ -130,6 +130,8 @@ class CacheBank(nn.Module):
         if counts is None:
             return None
         if not isinstance(counts, torch.Tensor):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("CacheBank: a graph cannot capture counts from the host; give them as a tensor on the device")
             values = [int(n) for n in counts]
             if len(values) != batch or any(n < 0 or n > T for n in values):
                 raise ValueError(f"counts must be {batch} numbers in [0, {T}], got {values}")

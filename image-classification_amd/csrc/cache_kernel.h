@@ -48,6 +48,9 @@ struct CacheView {
     int batch, heads, dim, rows, limit;      // rows: allocated (multiple of 64); limit: most rows that are used
 };
 
+// Rows in use of a sequence, whatever its buffer holds (a restored state may be anything).
+__device__ __forceinline__ int rows_used(const CacheView &c, int b) { return min(max(c.length[b], 0), c.limit); }
+
 // ---------------------------------------------------------------------------------------------------- element access
 template <int DT>
 __device__ __forceinline__ void load8(const void *p, float (&x)[8])
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
     const int chunks = WHOLE ? 1 : (p.T + TURN * TURNS - 1) / (TURN * TURNS);
     const int group = (int)(blockIdx.x / chunks), b = WHOLE ? (int)blockIdx.x : group / p.c.heads;
     const int first = WHOLE ? 0 : (int)(blockIdx.x % chunks) * TURN * TURNS, last = WHOLE ? p.c.heads * p.T : min(p.T, first + TURN * TURNS);
-    const int len = p.c.length[b], n = push_count(p, b, len);
+    const int len = rows_used(p.c, b), n = push_count(p, b, len);
 #pragma unroll WHOLE ? 1 : TURNS
     for (int r0 = first; r0 < last; r0 += TURN) {
         const int r = r0 + threadIdx.x / ROW;
@@ -231,9 +234,8 @@ __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
     if constexpr (WHOLE) {
         __syncthreads();
         if (threadIdx.x == 0) {
-            const int n = push_count(p, blockIdx.x, p.c.length[blockIdx.x]);
-            p.c.length[blockIdx.x] += n;
-            p.c.seen[blockIdx.x] += n;
+            p.c.length[b] = len + n;
+            p.c.seen[b] += n;
         }
     }
 }
@@ -243,8 +245,8 @@ __global__ void cache_advance_kernel(PushParams p)
 {
     const int b = blockIdx.x * 64 + threadIdx.x;
     if (b >= p.c.batch) return;
-    const int n = push_count(p, b, p.c.length[b]);
-    p.c.length[b] += n;
+    const int len = rows_used(p.c, b), n = push_count(p, b, len);
+    p.c.length[b] = len + n;
     p.c.seen[b] += n;
 }
 
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(256) void cache_longest_kernel(PushParams p, int *o
     int most = 0;
     for (int b = threadIdx.x; b < p.c.batch; b += 256) {
         const int n = p.counts ? p.counts[b] : p.T;
-        most = max(most, p.c.length[b] + (n < 0 ? 0 : n > p.T ? p.T : n));
+        most = max(most, rows_used(p.c, b) + (n < 0 ? 0 : n > p.T ? p.T : n));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
@@ -271,7 +273,7 @@ __global__ void cache_trim_kernel(CacheView c, const int *lengths, int length)
     if (b >= c.batch) return;
     int n = lengths ? lengths[b] : length;
     n = n < 0 ? 0 : n;
-    const int gone = c.length[b] - n;
+    const int gone = rows_used(c, b) - n;
     if (gone > 0) {
         c.length[b] = n;
         c.seen[b] -= gone;
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, uint4 *key
     const long long bh = blockIdx.x / chunks;
     const int d = threadIdx.x % SIDE, side = threadIdx.x / SIDE & 1, first = (int)(blockIdx.x % chunks) * TURN * CACHE_READ_TURNS;
     if (d * 8 >= c.dim) return;
-    const int len = c.length[bh / c.heads];
+    const int len = rows_used(c, (int)(bh / c.heads));
     const uint8_t *codes = (side ? c.value : c.key) + bh * c.rows * (W / 2) + d * 4;
     const uint8_t *scales = (side ? c.value_scale : c.key_scale) + (bh * (W / 32) + d / 4) * c.rows, *nans = c.key_scale + (bh * (W / 32) + d / 4) * c.rows;
     uint4 *out = (side ? value : key) + bh * c.limit * (c.dim / 8) + d;
@@ -445,6 +447,10 @@ struct UnitAt {                              // addresses of one lane within one
     __device__ __forceinline__ void load(long long u0, Unit<NB> &u) const
     {
         load_k(u0, u.k, u.ks);
+        load_v(u0, u);
+    }
+    __device__ __forceinline__ void load_v(long long u0, Unit<NB> &u) const
+    {
 #pragma unroll
         for (int e = 0; e < 8; ++e) load_value<NB>(v + (u0 + 16 * (e >> 2) + (e & 3)) * (16 * NB), u.v[e]);
 #pragma unroll
@@ -528,8 +534,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
     const int tile = (int)(id % p.tiles);
     const long long bh = id / p.tiles;
     const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
-    int len = p.c.length[b];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
 
     cb16x8 q[Q_LDS ? 1 : MT][NB][PQ];
@@ -579,7 +584,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
         if constexpr (Q_LDS) return __builtin_bit_cast(cb16x8, ((const uint4 *)s_both)[((m * NB + i) * PQ + k) * 64 + lane]);
         else return q[m][i][k];
     };
-    const auto compute = [&](int u0, const Unit<NB> &u) __attribute__((always_inline)) {
+    const auto compute = [&](int u0, Unit<NB> &u, int next) __attribute__((always_inline)) {
         cf32x4 s[MT][2], small[PQ > 1 ? MT : 1][2];               // products of the query's first piece, and of the others
 #pragma unroll
         for (int a = 0; a < 2; ++a)
@@ -601,6 +606,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 }
             if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
+        if (next < last) at.load_k((long long)next * 32, u.k, u.ks);
         if constexpr (PQ > 1) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -664,8 +670,10 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 }
             if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
+        if (next < last) at.load_v((long long)next * 32, u);
     };
-    // DEPTH units are on their way or in hand: a unit is computed about as fast as memory answers
+    // DEPTH units are on their way or in hand, and the next one's keys and values follow as soon as their registers are free: a unit
+    // is computed about as fast as memory answers.
     constexpr int DEPTH = MT * NB <= 4 ? 3 : NB < 8 && DT == CACHE_BF16 ? 2 : 1;
     Unit<NB> u[DEPTH];
 #pragma unroll
@@ -675,8 +683,7 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             if (un + 4 * d >= last) break;
-            compute((un + 4 * d) * 32, u[d]);
-            if (un + 4 * (d + DEPTH) < last) at.load((long long)(un + 4 * (d + DEPTH)) * 32, u[d]);
+            compute((un + 4 * d) * 32, u[d], un + 4 * (d + DEPTH));
         }
     }
 
@@ -835,8 +842,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
     const long long bh = blockIdx.x % bhs;
     const int rest = (int)(blockIdx.x / bhs), split = rest % p.nsplit, tile = p.tiles - 1 - rest / p.nsplit;
     const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
-    int len = p.c.length[b];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
 
     const int row = tile * ROWS + wave * 32 + c;
@@ -1106,8 +1112,7 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, j = lane >> 4;
     const long long bh = blockIdx.x / p.chunks;
     const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
-    int len = p.c.length[b];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
     const UnitAt<NB> at(p.c, bh, lane);
     for (int u0 = (int)(blockIdx.x % p.chunks) * 128 + wave * 32; u0 < len; u0 += p.chunks * 128) {
@@ -1170,8 +1175,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
     const long long bh = blockIdx.x % bhs;
     const int rest = (int)(blockIdx.x / bhs), piece = rest % p.rsplit, chunk = rest / p.rsplit;
     const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
-    int len = p.c.length[b];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
     const int tiles = (int)(((long long)n * p.G + QROWS - 1) / QROWS), per = (tiles + p.rsplit - 1) / p.rsplit;
     const char *const query = p.q + b * p.q_s[0] + (long long)h * p.G * p.q_s[1];
@@ -1322,8 +1326,7 @@ __global__ __launch_bounds__(256) void cache_weigh_add_kernel(CacheAttendParams 
 {
     const int bhs = p.c.batch * p.c.heads;
     const long long bh = blockIdx.x % bhs;
-    int len = p.c.length[bh / p.c.heads];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, (int)(bh / p.c.heads));
     const int step = (int)(gridDim.x / bhs) * 256;
     for (int slot = (int)(blockIdx.x / bhs) * 256 + threadIdx.x; slot < len; slot += step) {
         float w = p.c.weight[bh * p.c.rows + slot];
@@ -1337,8 +1340,7 @@ __global__ __launch_bounds__(256) void cache_weigh_scores_kernel(CacheAttendPara
 {
     const long long bh = blockIdx.x / p.chunks;
     const int b = (int)(bh / p.c.heads);
-    int len = p.c.length[b];
-    len = len > p.c.limit ? p.c.limit : len;
+    const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
     for (int slot = ((int)(blockIdx.x % p.chunks) * 256 + threadIdx.x) * 4; slot < len; slot += p.chunks * 1024) {
         float w[4] = {0, 0, 0, 0};
@@ -1516,8 +1518,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams
     __shared__ int s_pick[3];
     const long long bh = blockIdx.x;
     const int b = (int)(bh / p.c.heads), tid = threadIdx.x;
-    int n = p.c.length[b];
-    n = n > p.c.limit ? p.c.limit : n;
+    const int n = rows_used(p.c, b);
     if (n <= p.keep) {
         if (!p.in_place)
             for (int i = tid; i < n; i += EVICT_THREADS) p.pairs[bh * p.keep + i] = make_int2(i, i);
@@ -1565,8 +1566,7 @@ __global__ __launch_bounds__(256) void cache_move_kernel(EvictParams p, int chun
         }
     }
     if (chunk == 0 && threadIdx.x == 0 && bh % p.c.heads == 0) {
-        int n = p.c.length[b];
-        n = n > p.c.limit ? p.c.limit : n;
+        const int n = rows_used(p.c, b);
         p.into.length[b] = n < p.keep ? n : p.keep;
         if (!p.in_place) p.into.seen[b] = p.c.seen[b];
     }

@@ -568,6 +568,10 @@ def test_graph_capture_replays_like_eager():
             elif a.dim() > 1:
                 a, b = a[:, :, :n], b[:, :, :n]
             assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side), pytest.raises(RuntimeError, match="cannot capture counts"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            graphed.push("kv", *kv, counts=[1, 1])
     # the host does not know the lengths any more: it looks, and refuses what does not fit
     big = torch.zeros(B, H, k - keep + 1, dim, device="cuda")
     with pytest.raises(RuntimeError, match="do not fit"):
