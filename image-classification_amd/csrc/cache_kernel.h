@@ -1380,142 +1380,194 @@ __device__ __forceinline__ uint32_t evict_rank(float w, int position, int from)
 }
 
 constexpr int EVICT_THREADS = 1024, EVICT_BINS = 2048;
-constexpr int EVICT_RESIDENT = 36864;        // ranks of so many rows fit the 160 KB of shared memory beside the histogram
+constexpr int EVICT_LIST = 2048;             // rows of one bin of the first digit that are gathered for the other two
+constexpr int EVICT_RESIDENT = 32768;        // ranks of so many rows fit the shared memory beside the histogram and that list
+
+struct EvictShared {
+    int hist[EVICT_BINS];
+    uint32_t list[EVICT_LIST];
+    int2 wave[EVICT_THREADS / 64];
+    int pick[3], listed;
+};
 
 // Exclusive prefix sums of two numbers over the waves of the workgroup (one value a wave, from any lane of it).
-__device__ __forceinline__ int2 wave_scan2(int2 v, int2 *s_wave, int2 &all)
+__device__ __forceinline__ int2 wave_scan2(int2 v, EvictShared &sh, int2 &all)
 {
     const int wave = threadIdx.x >> 6;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_wave[wave] = v;
+    if ((threadIdx.x & 63) == 0) sh.wave[wave] = v;
     __syncthreads();
     int2 before = make_int2(0, 0);
     all = make_int2(0, 0);
 #pragma unroll
     for (int i = 0; i < EVICT_THREADS / 64; ++i) {
-        if (i < wave) before.x += s_wave[i].x, before.y += s_wave[i].y;
-        all.x += s_wave[i].x, all.y += s_wave[i].y;
+        if (i < wave) before.x += sh.wave[i].x, before.y += sh.wave[i].y;
+        all.x += sh.wave[i].x, all.y += sh.wave[i].y;
     }
     return before;
 }
 
-// The rank that the keep-th row has, by digits of 11, 11 and 10 bits, then the lists of what has to be copied: wave w goes over
-// the w-th sixteenth of the slots, 64 neighbours at a time, and counts with ballots.
+__device__ __forceinline__ int wave_sum(int x)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// One digit of a lane's rank into the histogram.  Equal neighbours (rows that nothing attended to yet) are counted once for the wave,
+// not 64 times in turn.
+__device__ __forceinline__ void count_digit(EvictShared &sh, bool in, int digit)
+{
+    const unsigned long long who = __ballot(in);
+    if (!who) return;
+    const int first = __builtin_amdgcn_readlane(digit, __ffsll((long long)who) - 1);
+    const unsigned long long same = __ballot(in && digit == first);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[first], __popcll(same));
+    if (in && digit != first) atomicAdd(&sh.hist[digit], 1);
+}
+
+__device__ __forceinline__ void clear_digits(EvictShared &sh)
+{
+    for (int i = threadIdx.x; i < EVICT_BINS; i += EVICT_THREADS) sh.hist[i] = 0;
+    __syncthreads();
+}
+
+// The bin that holds the left-th largest (bins from the top, two a thread): its digit, how many of it stay, how many it has.
+__device__ __forceinline__ void pick_digit(EvictShared &sh, int left)
+{
+    __syncthreads();
+    const int lane = threadIdx.x & 63, top = EVICT_BINS - 1 - 2 * threadIdx.x, a = sh.hist[top], b = sh.hist[top - 1];
+    int sum = a + b;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(sum, d);
+        if (lane >= d) sum += v;
+    }
+    int2 all;
+    const int above = wave_scan2(make_int2(__builtin_amdgcn_readlane(sum, 63), 0), sh, all).x + sum - a - b;
+    if (above < left && above + a + b >= left) {
+        const bool second = above + a < left;
+        sh.pick[0] = second ? top - 1 : top;
+        sh.pick[1] = left - above - (second ? a : 0);
+        sh.pick[2] = second ? b : a;
+    }
+    __syncthreads();
+}
+
+// Calls f(row, its rank) for all rows of a stretch, 64 neighbours a wave at a time, four ranks on their way; rows past the end have
+// rank 0 and are told by their number.
+template <int STEP, typename Rank, typename F>
+__device__ __forceinline__ void for_ranks(int lo, int hi, Rank rank, F f)
+{
+    const int lane = threadIdx.x & 63;
+    for (int i0 = lo; i0 < hi; i0 += 4 * STEP) {
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = i0 + k * STEP + lane < hi ? rank(i0 + k * STEP + lane) : 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f(i0 + k * STEP + lane, r[k]);
+    }
+}
+
+// The rank that the keep-th row has, by digits of 11, 11 and 10 bits (the first one may be counted already), then the lists of what has
+// to be copied: wave w goes over the w-th sixteenth of the slots and counts with ballots.
 template <typename Rank>
-__device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, int n, Rank rank, int *s_hist, int2 *s_wave, int *s_pick)
+__device__ __forceinline__ void select_rows(const EvictParams &p, long long bh, int n, Rank rank, EvictShared &sh, bool counted)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keep = p.keep;
     int2 *pairs = p.pairs + bh * keep;
-    uint32_t prefix = 0, known = 0;
-    int left = keep;
-#pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t mask = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) s_hist[i] = 0;
-        __syncthreads();
-        for (int i0 = wave * 64; i0 < n; i0 += 4 * EVICT_THREADS) {
-            uint32_t r[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r[k] = i0 + k * EVICT_THREADS + lane < n ? rank(i0 + k * EVICT_THREADS + lane) : 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool in = i0 + k * EVICT_THREADS + lane < n && (r[k] & known) == prefix;
-                const int digit = (int)((r[k] >> shift) & mask);
-                // equal neighbours (rows that nothing attended to yet) are counted once for the wave, not 64 times in turn
-                const unsigned long long who = __ballot(in);
-                if (who) {
-                    const int first = __builtin_amdgcn_readlane(digit, __ffsll((long long)who) - 1);
-                    const unsigned long long same = __ballot(in && digit == first);
-                    if (lane == 0) atomicAdd(&s_hist[first], __popcll(same));
-                    if (in && digit != first) atomicAdd(&s_hist[digit], 1);
-                }
-            }
-        }
-        __syncthreads();
-        // the bin that holds the left-th largest: bins from the top, two a thread
-        const int top = EVICT_BINS - 1 - 2 * tid, a = s_hist[top], b = s_hist[top - 1];
-        int sum = a + b;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(sum, d);
-            if (lane >= d) sum += v;
-        }
-        int2 all;
-        const int total = __builtin_amdgcn_readlane(sum, 63);
-        const int above = wave_scan2(make_int2(total, 0), s_wave, all).x + sum - a - b;
-        if (above < left && above + a + b >= left) {
-            const bool second = above + a < left;
-            s_pick[0] = second ? top - 1 : top;
-            s_pick[1] = left - above - (second ? a : 0);
-            s_pick[2] = second ? b : a;                           // rows in it
-        }
-        __syncthreads();
-        prefix |= (uint32_t)s_pick[0] << shift;
-        left = s_pick[1];
-        known |= mask << shift;
+    if (!counted) {
+        clear_digits(sh);
+        for_ranks<EVICT_THREADS>(wave * 64, n, rank, [&](int i, uint32_t r) { count_digit(sh, i < n, (int)(r >> 21)); });
+    }
+    pick_digit(sh, keep);
+    uint32_t prefix = (uint32_t)sh.pick[0] << 21;
+    int left = sh.pick[1];
+    const int listed = sh.pick[2];
+    const bool gather = listed <= EVICT_LIST;
+    if (tid == 0) sh.listed = 0;
+    clear_digits(sh);
+    if (gather) {                            // the rows of that bin, in any order: the other digits look at them alone
+        for_ranks<EVICT_THREADS>(wave * 64, n, rank, [&](int i, uint32_t r) {
+            const bool in = i < n && (r & 0xffe00000u) == prefix;
+            const unsigned long long who = __ballot(in);
+            if (!who) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
+            if (in) sh.list[at] = r;
+        });
         __syncthreads();
     }
-    // rows above the edge stay, and of those on it the `left` lowest slots
+#pragma unroll
+    for (int pass = 1; pass < 3; ++pass) {
+        const int shift = pass == 1 ? 10 : 0;
+        const uint32_t mask = pass == 1 ? 2047u : 1023u, known = pass == 1 ? 0xffe00000u : 0xfffffc00u;
+        if (pass == 2) clear_digits(sh);
+        const auto count = [&](int i, int end, uint32_t r) { count_digit(sh, i < end && (r & known) == prefix, (int)((r >> shift) & mask)); };
+        if (gather) for_ranks<EVICT_THREADS>(wave * 64, listed, [&](int i) { return sh.list[i]; }, [&](int i, uint32_t r) { count(i, listed, r); });
+        else for_ranks<EVICT_THREADS>(wave * 64, n, rank, [&](int i, uint32_t r) { count(i, n, r); });
+        pick_digit(sh, left);
+        prefix |= (uint32_t)sh.pick[0] << shift;
+        left = sh.pick[1];
+    }
+    // rows above the edge stay, and of those on it the `left` lowest slots: in the usual case all of them
     const uint32_t edge = prefix;
+    const bool all_ties = sh.pick[2] == left;
     const int seg = ((n + EVICT_THREADS - 1) / EVICT_THREADS) * 64, lo = min(n, wave * seg), hi = min(n, lo + seg);
     const unsigned long long below = (1ull << lane) - 1;
-    const bool all_ties = s_pick[2] == left;                      // the usual case: every row on the edge stays
     int2 all;
     int eq0 = 0;
     if (!all_ties) {
         int eq = 0;
-        for (int i0 = lo; i0 < hi; i0 += 64) eq += __popcll(__ballot(i0 + lane < hi && rank(i0 + lane) == edge));
-        eq0 = wave_scan2(make_int2(eq, 0), s_wave, all).x;
+        for_ranks<64>(lo, hi, rank, [&](int i, uint32_t r) { eq += i < hi && r == edge; });
+        eq0 = wave_scan2(make_int2(wave_sum(eq), 0), sh, all).x;
     }
-    int2 off = make_int2(0, 0);              // freed slots below keep, kept rows from there on
-    int base = 0;                            // pairs before those of the freed slots
-#pragma unroll
-    for (int write = 0; write < 2; ++write) {
-        int at = eq0, holes = 0, tails = 0;
-        for (int i1 = lo; i1 < hi; i1 += 256) {
-            uint32_t rs[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) rs[k] = i1 + 64 * k + lane < hi ? rank(i1 + 64 * k + lane) : 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i1 + 64 * k + lane;
-                const uint32_t r = rs[k];
-                bool kept = i < hi && r >= edge;
-                if (!all_ties) {
-                    const unsigned long long on = __ballot(i < hi && r == edge);
-                    kept = i < hi && (r > edge || (r == edge && at + __popcll(on & below) < left));
-                    at += __popcll(on);
-                }
-                const bool hole = i < hi && i < keep && !kept, tail = i >= keep && kept;
-                const unsigned long long h = __ballot(hole), t = __ballot(tail);
-                if (write) {
-                    const int nh = off.x + holes + __popcll(h & below), nt = off.y + tails + __popcll(t & below);
-                    if (hole) pairs[base + nh].x = i;
-                    if (tail) pairs[base + nt].y = i;
-                    if (base && i < keep && kept) pairs[i - nh] = make_int2(i, i);
-                }
-                holes += __popcll(h);
-                tails += __popcll(t);
-            }
+    int at = eq0;                            // rows on the edge before this wave's next 64
+    const auto kept_at = [&](int i, uint32_t r) {
+        if (all_ties) return i < hi && r >= edge;
+        const unsigned long long on = __ballot(i < hi && r == edge);
+        const bool kept = i < hi && (r > edge || (r == edge && at + __popcll(on & below) < left));
+        at += __popcll(on);
+        return kept;
+    };
+    int holes = 0, tails = 0;                // freed slots below keep, kept rows from there on
+    for_ranks<64>(lo, hi, rank, [&](int i, uint32_t r) {
+        const bool kept = kept_at(i, r);
+        holes += i < hi && i < keep && !kept;
+        tails += i >= keep && kept;
+    });
+    const int2 off = wave_scan2(make_int2(wave_sum(holes), wave_sum(tails)), sh, all);
+    const int base = p.in_place ? 0 : keep - all.x;               // pairs before those of the freed slots: rows that stay where they are
+    if (tid == 0) p.count[bh] = p.in_place ? all.x : keep;
+    at = eq0, holes = off.x, tails = off.y;
+    for_ranks<64>(lo, hi, rank, [&](int i, uint32_t r) {
+        const bool kept = kept_at(i, r);
+        const int i0 = __builtin_amdgcn_readfirstlane(i);
+        if (i0 < keep) {
+            const unsigned long long h = __ballot(i < hi && i < keep && !kept);
+            const int nh = holes + __popcll(h & below);
+            if (h >> lane & 1) pairs[base + nh].x = i;
+            else if (base && i < keep && kept) pairs[i - nh] = make_int2(i, i);
+            holes += __popcll(h);
         }
-        if (!write) {
-            off = wave_scan2(make_int2(holes, tails), s_wave, all);
-            base = p.in_place ? 0 : keep - all.x;
-            if (tid == 0) p.count[bh] = p.in_place ? all.x : keep;
+        if (i0 + 63 >= keep) {
+            const unsigned long long t = __ballot(i >= keep && kept);
+            if (t >> lane & 1) pairs[base + tails + __popcll(t & below)].y = i;
+            tails += __popcll(t);
         }
-    }
+    });
 }
 
 // One workgroup per (sequence, head).  The freed slots below `keep` take, in ascending order, the kept rows from above: in place
 // no row is read that another one is written to, and no more rows move than left.  Ranks are built in one pass over weights and
-// positions and stay in shared memory where they fit; `resident` of them do.
+// positions, all of its loads at once, and stay in shared memory where they fit; `resident` of them do.  (32 banks of 24 k rows: 203 us
+// with a pass over memory for each of four digits and a thread a stretch of slots, 38 us with ranks in shared memory and loads one
+// after the other.)
 __global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams p, int resident)
 {
     extern __shared__ uint32_t s_rank[];
-    __shared__ int s_hist[EVICT_BINS];
-    __shared__ int2 s_wave[EVICT_THREADS / 64];
-    __shared__ int s_pick[3];
+    __shared__ EvictShared sh;
     const long long bh = blockIdx.x;
     const int b = (int)(bh / p.c.heads), tid = threadIdx.x;
     const int n = rows_used(p.c, b);
@@ -1529,16 +1581,30 @@ __global__ __launch_bounds__(EVICT_THREADS) void cache_select_kernel(EvictParams
     const float *w = p.c.weight + bh * p.c.rows;
     const int *pos = p.c.position + bh * p.c.rows;
     if (n <= resident) {
-#pragma unroll 4
-        for (int i = tid * 4; i < n; i += EVICT_THREADS * 4) {        // rows are allocated in 64s: whole vectors
-            const float4 x = *(const float4 *)(w + i);
-            const int4 y = *(const int4 *)(pos + i);
-            *(uint4 *)(s_rank + i) = make_uint4(evict_rank(x.x, y.x, from), evict_rank(x.y, y.y, from), evict_rank(x.z, y.z, from), evict_rank(x.w, y.w, from));
+        constexpr int LOADS = EVICT_RESIDENT / (EVICT_THREADS * 4);
+        float4 x[LOADS];
+        int4 y[LOADS];
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {                         // rows are allocated in 64s: whole vectors
+            const int i = (tid + k * EVICT_THREADS) * 4;
+            x[k] = i < n ? *(const float4 *)(w + i) : make_float4(0, 0, 0, 0);
+            y[k] = i < n ? *(const int4 *)(pos + i) : make_int4(0, 0, 0, 0);
         }
-        __syncthreads();
-        select_rows(p, bh, n, [&](int i) { return s_rank[i]; }, s_hist, s_wave, s_pick);
+        clear_digits(sh);
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {
+            const int i = (tid + k * EVICT_THREADS) * 4;
+            if (__builtin_amdgcn_readfirstlane(i) >= n) break;
+            const uint4 r = make_uint4(evict_rank(x[k].x, y[k].x, from), evict_rank(x[k].y, y[k].y, from), evict_rank(x[k].z, y[k].z, from), evict_rank(x[k].w, y[k].w, from));
+            if (i < n) *(uint4 *)(s_rank + i) = r;
+            count_digit(sh, i < n, (int)(r.x >> 21));
+            count_digit(sh, i + 1 < n, (int)(r.y >> 21));
+            count_digit(sh, i + 2 < n, (int)(r.z >> 21));
+            count_digit(sh, i + 3 < n, (int)(r.w >> 21));
+        }
+        select_rows(p, bh, n, [&](int i) { return s_rank[i]; }, sh, true);
     } else
-        select_rows(p, bh, n, [&](int i) { return evict_rank(w[i], pos[i], from); }, s_hist, s_wave, s_pick);
+        select_rows(p, bh, n, [&](int i) { return evict_rank(w[i], pos[i], from); }, sh, false);
 }
 
 // Copies the rows of the lists.  W / 8 lanes a row: a quarter of them for each of key, value, their scales; 16 bytes a lane.

@@ -436,7 +436,7 @@ def _set_weights(bank, ref, rs, style):
 
 @gpu
 @pytest.mark.parametrize("style", ["spread", "ties", "equal", "special"])
-@pytest.mark.parametrize("dim,fill,keep,recent", [(64, 1, 1, 0), (64, 70, 1, 1), (128, 300, 299, 10), (128, 300, 64, 64), (256, 1000, 37, 5), (72, 5000, 4500, 300), (64, 2500, 1200, 0), (32, 9000, 8500, 100), (64, 20000, 10000, 7), (8, 40000, 15000, 70)])
+@pytest.mark.parametrize("dim,fill,keep,recent", [(64, 1, 1, 0), (64, 70, 1, 1), (128, 300, 299, 10), (128, 300, 64, 64), (256, 1000, 37, 5), (72, 5000, 4500, 300), (64, 2500, 1200, 0), (32, 9000, 8500, 100), (64, 20000, 10000, 7), (8, 40000, 15000, 70), (8, 32768, 700, 3), (8, 32769, 31000, 1)])
 def test_evict_in_place_and_into(style, dim, fill, keep, recent):
     rs = np.random.RandomState(fill + keep)
     B, H = 3, 2
