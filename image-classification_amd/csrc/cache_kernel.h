@@ -816,21 +816,13 @@ __device__ __forceinline__ void load_query32(const CacheAttendParams &p, int b, 
     split_pieces<P>(x, q);
 }
 
-// x + the sum of the two halves of a word of bf16, in float32 and one instruction.
-__device__ __forceinline__ float add_pair(uint32_t pair, float x)
-{
-    const uint32_t ones = 0x3f803f80u;
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(cb16x2, pair), __builtin_bit_cast(cb16x2, ones), x, false);
-}
-
 // How much a score may pass the reference of the exponent (in powers of two) before sums are rescaled: float32 and bf16 have the
 // range, and with it the reference hardly ever moves after the first tile.
 constexpr float CACHE_SLACK = 16.f;
 
 // Pieces of the probabilities: one for bf16 (2^-8 of each p at most, as much as the result's own rounding may be), as many as the
-// query's for the others.  The denominator sums the rounded p of bf16, a pair an instruction; where attention sums divide by it too
-// (EXACT) and for the other types it sums p as it is (prompt of 4096, 32 heads on 8: 164 us with pairs, 194 us without).
-template <int DT, int NB, int WAVES, bool EXACT>
+// query's for the others.  The denominator sums them unrounded: attention sums are divided by it too.
+template <int DT, int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE_F32 ? 1 : 2) void cache_attend_tile_kernel(CacheAttendParams p)
 {
     constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, PP = PQ, ROWS = 32 * WAVES, TOKENS = 16 * WAVES, SUB = TOKENS / 32;
@@ -926,14 +918,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     x[e] = __builtin_amdgcn_exp2f(fmaf(s[sq >> 1][(sq & 1) * 8 + e], p.c2, off));
-                    if constexpr (EXACT) sum += x[e];
+                    sum += x[e];
                 }
                 cb16x8 pf[PP];
                 split_pieces<PP, false>(x, pf);
-                if constexpr (!EXACT) {
-                    const uint4 w = __builtin_bit_cast(uint4, pf[0]);
-                    sum = add_pair(w.x, add_pair(w.y, add_pair(w.z, add_pair(w.w, sum))));
-                }
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     const cb16x8 vf = __builtin_bit_cast(cb16x8, values[(sq * NB + i) * 64 + lane]);
@@ -1168,7 +1156,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
 {
     constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, RT = 2 * SK * PQ > 64 ? 1 : 2, QROWS = 32 * RT;
     constexpr int MINE = RT * SK / 8;                             // fragments of a query tile (RT SK) that a wave loads
-    static_assert(MINE * 8 == RT * SK, "eight waves");
+    static_assert(MINE * 8 == RT * SK && (RT == 1 || SK == 4 * MINE), "eight waves, each with steps of one 32 rows");
     __shared__ uint4 s_q[2][RT * SK * PQ][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
     const int bhs = p.c.batch * p.c.heads;
@@ -1178,8 +1166,20 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
     const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);
     const int tiles = (int)(((long long)n * p.G + QROWS - 1) / QROWS), per = (tiles + p.rsplit - 1) / p.rsplit;
+    // A wave loads fragments of one 32 rows of a tile (its row c), steps `step` on; dims that pad a row read its first ones, which
+    // meet zeros of the bank.
+    const int mine32 = RT == 2 ? wave >> 2 : 0, step = wave * MINE % SK, real_rows_all = n * p.G;
     const char *const query = p.q + b * p.q_s[0] + (long long)h * p.G * p.q_s[1];
     const int dt = QROWS / p.G, dg = QROWS - dt * p.G;            // from a tile's row to the next one's, without a division
+    const long long ahead = dt * p.q_s[2] + dg * p.q_s[1], wrap = p.q_s[2] - p.G * p.q_s[1];
+    const char *const final = query + (long long)max(n - 1, 0) * p.q_s[2] + (p.G - 1) * p.q_s[1];
+    int at_dim[MINE];
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+        const int d = l * 16 * NB + (step + m) * 8;
+        at_dim[m] = d < p.c.dim ? d * elem_bytes<DT>() : 0;
+    }
+    const float2 *const norms = p.norm + bh * p.R;
     for (int w0 = chunk * 256; w0 < len; w0 += p.chunks * 256) {
         const int u0 = w0 + wave * 32;
         cb16x8 kf[SK];
@@ -1204,80 +1204,86 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
         const int first = max(piece * per, (int)min((long long)tiles, (long long)t_lo * p.G / QROWS)), last = min(tiles, (piece + 1) * per);
         const int border = max(first, (int)min((long long)last, ((long long)t_all * p.G + QROWS - 1) / QROWS));
         if (first < last) {
-            int t[RT], g[RT];                                     // token and head of rows c, 32 + c of the tile that is loaded next
-#pragma unroll
-            for (int a = 0; a < RT; ++a) {
-                t[a] = (first * QROWS + 32 * a + c) / p.G;
-                g[a] = first * QROWS + 32 * a + c - t[a] * p.G;
-            }
+            int next = first * QROWS;                             // the tile that is loaded next, by its first row
+            int g = (next + 32 * mine32 + c) % p.G;
+            const char *row = query + (long long)((next + 32 * mine32 + c) / p.G) * p.q_s[2] + g * p.q_s[1];
             uint4 mine[MINE * PQ];
             float2 norm[3][RT];                                   // of the tile in hand, the next, the one loaded
-            int see[3][RT];
+            // Rows past the last real one repeat it and count zero times.
             const auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int a = 0; a < RT; ++a) {
-                    const bool real = t[a] < n;
-                    see[2][a] = real ? visible(t[a], n, len, p.causal) : 0;
-                    const float2 row = p.norm[bh * p.R + (real ? t[a] * p.G + g[a] : 0)];
-                    norm[2][a] = make_float2(real ? -row.x : 0.f, real ? row.y : 0.f);
+                    const int r = next + 32 * a + c;
+                    norm[2][a] = norms[min(r, real_rows_all - 1)];
+                    norm[2][a].x = -norm[2][a].x;
+                    norm[2][a].y = r < real_rows_all ? norm[2][a].y : 0.f;
                 }
+                const char *from = next + 32 * mine32 + c < real_rows_all ? row : final;
 #pragma unroll
                 for (int m = 0; m < MINE; ++m) {
-                    const int f = wave * MINE + m, a = f / SK, d = l * 16 * NB + f % SK * 8;
-                    const int ta = a ? t[RT - 1] : t[0], ga = a ? g[RT - 1] : g[0];
-                    const bool in = ta < n && d < p.c.dim;
-                    const char *src = query + (in ? (long long)ga * p.q_s[1] + ta * p.q_s[2] + (long long)d * elem_bytes<DT>() : 0);
                     if constexpr (DT == CACHE_BF16) {
-                        const uint4 x = *(const uint4 *)src;
-                        mine[m] = make_uint4(in ? x.x : 0, in ? x.y : 0, in ? x.z : 0, in ? x.w : 0);
+                        const uint4 x = *(const uint4 *)(from + at_dim[m]);
+                        mine[m] = make_uint4(x.x, x.y, x.z, x.w);             // (copied whole, the array went to memory)
                     } else {
                         float x[8];
-                        load8<DT>(src, x);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = in ? x[i] : 0.f;
+                        load8<DT>(from + at_dim[m], x);
                         cb16x8 q[PQ];
                         split_pieces<PQ>(x, q);
 #pragma unroll
                         for (int k = 0; k < PQ; ++k) mine[m * PQ + k] = __builtin_bit_cast(uint4, q[k]);
                     }
                 }
-#pragma unroll
-                for (int a = 0; a < RT; ++a) {
-                    t[a] += dt, g[a] += dg;
-                    if (g[a] >= p.G) g[a] -= p.G, ++t[a];
-                }
+                next += QROWS;
+                g += dg;
+                row += ahead;
+                if (g >= p.G) g -= p.G, row += wrap;
             };
             const auto leave = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
                 for (int m = 0; m < MINE * PQ; ++m) s_q[(tile - first) & 1][wave * MINE * PQ + m][lane] = mine[m];
 #pragma unroll
-                for (int a = 0; a < RT; ++a) norm[0][a] = norm[1][a], norm[1][a] = norm[2][a], see[0][a] = see[1][a], see[1][a] = see[2][a];
+                for (int a = 0; a < RT; ++a) norm[0][a] = norm[1][a], norm[1][a] = norm[2][a];
             };
-            const auto product = [&](int tile, cf32x16 (&s)[RT]) __attribute__((always_inline)) {
+            // Scores of tile `tile + 1` (past the last one: of whatever is there, never used) into `ahead`, beside the exponentials of
+            // tile `tile`, whose scores are in `s` (NOW false: without them).  The order is fixed: a matrix instruction, the operand four
+            // further on, and the vector instructions that fit beside; left alone, the compiler reads each operand right before its use
+            // and puts all of one kind before all of the other, and a wave issues in order.  The smaller pieces of the query come first.
+            constexpr int FRAGS = RT * SK * PQ, RING = 4;
+            const auto both = [&](int tile, cf32x16 (&s)[RT], cf32x16 (&ahead)[RT], auto now, auto masked) __attribute__((always_inline)) {
+                const uint4 (*const from)[64] = s_q[(tile + 1 - first) & 1];
+                const auto operand = [&](int f) __attribute__((always_inline)) {      // f: piece (descending), step, 32 rows
+                    const int k = PQ - 1 - f / (RT * SK), i = f / RT % SK, a = f % RT;
+                    return __builtin_bit_cast(cb16x8, from[(a * SK + i) * PQ + k][lane]);
+                };
+                cb16x8 ring[RING];
 #pragma unroll
-                for (int a = 0; a < RT; ++a)
+                for (int f = 0; f < RING; ++f) ring[f] = operand(f);
+                int left[RT];                                     // slots from this lane's first that its row of the tile sees
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
-                // the smaller pieces first
+                for (int a = 0; a < RT; ++a) {
+                    left[a] = 0;
+                    if constexpr (decltype(masked)::value) left[a] = visible((tile * QROWS + 32 * a + c) / p.G, n, len, p.causal) - u0 - 4 * l;
 #pragma unroll
-                for (int k = PQ - 1; k >= 0; --k)
+                    for (int r = 0; r < 16; ++r) ahead[a][r] = 0.f;
+                }
 #pragma unroll
-                    for (int i = 0; i < SK; ++i)
+                for (int f = 0; f < FRAGS; ++f) {
+                    ahead[f % RT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[f / RT % SK], ring[f % RING], ahead[f % RT], 0, 0, 0);
+                    if (f + RING < FRAGS) ring[f % RING] = operand(f + RING);
+                    if constexpr (decltype(now)::value) {
 #pragma unroll
-                        for (int a = 0; a < RT; ++a)
-                            s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], __builtin_bit_cast(cb16x8, s_q[(tile - first) & 1][(a * SK + i) * PQ + k][lane]), s[a], 0, 0, 0);
-            };
-            // scores of the next tile (past the last one: of whatever is there, never used) beside the exponentials of this one
-            const auto step = [&](int tile, cf32x16 (&s)[RT], cf32x16 (&ahead)[RT], auto masked) __attribute__((always_inline)) {
-                product(tile + 1, ahead);
-#pragma unroll
-                for (int a = 0; a < RT; ++a)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, norm[0][a].x)), more = fmaf(x, norm[0][a].y, w[r]);
-                        if constexpr (decltype(masked)::value) w[r] = u0 + 8 * (r >> 2) + 4 * l + (r & 3) < see[0][a] ? more : w[r];
-                        else w[r] = more;
+                        for (int e = f * 16 * RT / FRAGS; e < (f + 1) * 16 * RT / FRAGS; ++e) {
+                            const int a = e / 16, r = e % 16;
+                            const float x = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.c2, norm[0][a].x)), more = fmaf(x, norm[0][a].y, w[r]);
+                            if constexpr (decltype(masked)::value) w[r] = 8 * (r >> 2) + (r & 3) < left[a] ? more : w[r];
+                            else w[r] = more;
+                        }
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            const auto step = [&](int tile, cf32x16 (&s)[RT], cf32x16 (&ahead)[RT], auto masked) __attribute__((always_inline)) {
+                both(tile, s, ahead, std::true_type(), masked);
                 leave(tile);                                      // tile + 2, into the buffer that this tile had
                 fetch();
                 __syncthreads();
@@ -1303,7 +1309,7 @@ __global__ __launch_bounds__(512, 2) void cache_weigh_tile_kernel(CacheAttendPar
             leave(first + 1);
             fetch();
             __syncthreads();
-            product(first, s0);
+            both(first - 1, s1, s0, std::false_type(), std::false_type());
             __syncthreads();                                      // the first step writes where this one read
             run(border, std::true_type());
             run(last, std::false_type());

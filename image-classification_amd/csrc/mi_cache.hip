@@ -144,14 +144,14 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     return a;
 }
 
-template <int DT, int NB, int WAVES, bool EXACT>
+template <int DT, int NB, int WAVES>
 hipError_t launch_tile(const mi::CacheAttendParams &p, dim3 grid, hipStream_t s)
 {
     const size_t lds = (size_t)NB * WAVES * 4 * 1024;      // two tiles of 16 WAVES rows, keys and values in bf16
     static std::atomic<uint64_t> done{0};
-    const hipError_t e = ensure_dynamic_lds(mi::cache_attend_tile_kernel<DT, NB, WAVES, EXACT>, lds, done);
+    const hipError_t e = ensure_dynamic_lds(mi::cache_attend_tile_kernel<DT, NB, WAVES>, lds, done);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((mi::cache_attend_tile_kernel<DT, NB, WAVES, EXACT>), grid, dim3(64 * WAVES), lds, s, p);
+    hipLaunchKernelGGL((mi::cache_attend_tile_kernel<DT, NB, WAVES>), grid, dim3(64 * WAVES), lds, s, p);
     return hipGetLastError();
 }
 
@@ -162,11 +162,8 @@ hipError_t launch_attend(const mi::CacheAttendParams &p, const AttendPlan &a, in
     const dim3 grid((unsigned)(bh * a.tiles * a.nsplit));
     if (a.tiled) {
         hipError_t e;
-        if constexpr (DT == mi::CACHE_BF16) {
-            if constexpr (NB < 8) e = a.waves == 8 ? (accumulate ? launch_tile<DT, NB, 8, true>(p, grid, s) : launch_tile<DT, NB, 8, false>(p, grid, s))
-                                                   : (accumulate ? launch_tile<DT, NB, 4, true>(p, grid, s) : launch_tile<DT, NB, 4, false>(p, grid, s));
-            else e = accumulate ? launch_tile<DT, NB, 4, true>(p, grid, s) : launch_tile<DT, NB, 4, false>(p, grid, s);
-        } else e = launch_tile<DT, NB, 4, true>(p, grid, s);
+        if constexpr (DT == mi::CACHE_BF16 && NB < 8) e = a.waves == 8 ? launch_tile<DT, NB, 8>(p, grid, s) : launch_tile<DT, NB, 4>(p, grid, s);
+        else e = launch_tile<DT, NB, 4>(p, grid, s);
         if (e != hipSuccess) return e;
     } else if (a.mt == 1) hipLaunchKernelGGL((mi::cache_attend_kernel<DT, NB, 1>), grid, dim3(256), 0, s, p);
     if constexpr (NB < 8)
