@@ -827,6 +827,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
 {
     constexpr int W = 32 * NB, SK = 2 * NB, PQ = Pieces<DT>::N, PP = PQ, ROWS = 32 * WAVES, TOKENS = 16 * WAVES, SUB = TOKENS / 32;
     constexpr int KF = SUB * SK, VF = WAVES * NB;                 // fragments of a tile
+    constexpr int RING = 4;                  // operands on their way: read right before its use, one waits for shared memory longer than for the matrix core
     extern __shared__ uint4 s_tile[];        // [2][KF + VF][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
     // heads innermost (a head's bank stays in one die's cache where heads are a multiple of 8), the longest rows first
@@ -874,17 +875,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
             for (int tt = 0; tt < SUB; ++tt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[tt][r] = small[PQ > 1 ? tt : 0][r] = 0.f;
+            const auto operand = [&](int f) __attribute__((always_inline)) { return __builtin_bit_cast(cb16x8, keys[(f % SUB * SK + f / SUB) * 64 + lane]); };
+            cb16x8 ring[RING];
 #pragma unroll
-            for (int i = 0; i < SK; ++i)
+            for (int f = 0; f < RING; ++f) ring[f] = operand(f);
 #pragma unroll
-                for (int tt = 0; tt < SUB; ++tt) {
-                    const cb16x8 kf = __builtin_bit_cast(cb16x8, keys[(tt * SK + i) * 64 + lane]);
+            for (int f = 0; f < SUB * SK; ++f) {
+                const int i = f / SUB, tt = f % SUB;
 #pragma unroll
-                    for (int k = 0; k < PQ; ++k) {
-                        cf32x16 &to = k ? small[PQ > 1 ? tt : 0] : s[tt];
-                        to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i][k], to, 0, 0, 0);
-                    }
+                for (int k = 0; k < PQ; ++k) {
+                    cf32x16 &to = k ? small[PQ > 1 ? tt : 0] : s[tt];
+                    to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[f % RING], q[i][k], to, 0, 0, 0);
                 }
+                if (f + RING < SUB * SK) ring[f % RING] = operand(f + RING);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if constexpr (PQ > 1) {
 #pragma unroll
                 for (int tt = 0; tt < SUB; ++tt) s[tt] += small[tt];
@@ -912,6 +917,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
             const uint4 *values = s_tile + ((un - first) & 1) * (KF + VF) * 64 + KF * 64;
             const float off = ref == -INFINITY ? 0.f : -ref;
             float sum = 0.f;
+            const auto operand = [&](int f) __attribute__((always_inline)) { return __builtin_bit_cast(cb16x8, values[f * 64 + lane]); };
+            cb16x8 ring[RING];
+#pragma unroll
+            for (int f = 0; f < RING; ++f) ring[f] = operand(f);
 #pragma unroll
             for (int sq = 0; sq < 2 * SUB; ++sq) {
                 float x[8];
@@ -924,9 +933,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
                 split_pieces<PP, false>(x, pf);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    const cb16x8 vf = __builtin_bit_cast(cb16x8, values[(sq * NB + i) * 64 + lane]);
+                    const int f = sq * NB + i;
 #pragma unroll
-                    for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[i], 0, 0, 0);
+                    for (int k = 0; k < PP; ++k) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[f % RING], pf[k], o[i], 0, 0, 0);
+                    if (f + RING < 2 * SUB * NB) ring[f % RING] = operand(f + RING);
                 }
             }
             total.add(sum);
