@@ -888,7 +888,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
                     to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[f % RING], q[i][k], to, 0, 0, 0);
                 }
                 if (f + RING < SUB * SK) ring[f % RING] = operand(f + RING);
-                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (NB > 2) __builtin_amdgcn_sched_barrier(0);      // (64 dims: 406 us for 8192 rows in this order, 345 us in the compiler's)
             }
             if constexpr (PQ > 1) {
 #pragma unroll
