@@ -1,7 +1,8 @@
 """image-classification_amd -- MI355X-native feature-bank similarity path.
 
 One hot path of sailist/image-classification, rebuilt for gfx950: the weighted-kNN monitor
-(``models/knn.py``) and the MoCo queue (``models/memory_bank.py``, ``track_ssl/moco.py``).
+(``models/knn.py``) and the MoCo queue (``models/memory_bank.py``, ``track_ssl/moco.py``); beside their banks, :class:`CacheBank`
+holds keys and values in 4 bits, reads them by softmax attention and evicts by what attention they got.
 Import as ``image_classification_amd`` (alias module at the repository root)."""
 from . import _lib
 from . import module_utils
