@@ -1,7 +1,7 @@
 // cache_kernel.h -- a bank of key / value rows held in 4 bits: quantising append, softmax attention, eviction.
 //
-// Held format (OCP microscaling FP4).  A row of `dim` values is padded with zeros to W = 64 NB / 2 ... in {64, 128, 256} and
-// cut into blocks of 32.  A block has one scale 2^e, e the smallest integer with max|x| <= 7 * 2^e (7 = the half step above
+// Held format (OCP microscaling FP4).  A row of `dim` values is padded with zeros to W = 32 NB in {64, 128, 256} and cut
+// into blocks of 32.  A block has one scale 2^e, e the smallest integer with max|x| <= 7 * 2^e (7 = the half step above
 // the largest element 6, so that the largest value of a block is never further off than half a step of its binade), clamped
 // to [-126, 125] and stored as the byte e + 127.  Elements are x / 2^e on E2M1 (0 .5 1 1.5 2 3 4 6, sign bit), nearest even,
 // saturating; two a byte, the even one in the low four bits.  Every element times its scale is exact in bf16, which is what
@@ -335,7 +335,7 @@ struct CacheAttendParams {
     long long out_s[3];
     const int *counts;                       // real query rows of each sequence, or null: all T
     int T, G, causal;                        // G query heads read one head of the bank
-    int R, tiles;                            // R = T G rows per (sequence, head), row = t G + g; tiles of MT * 16 of them
+    int R, tiles;                            // R = T G rows per (sequence, head), row = t G + g; tiles of 16 MT or 32 WAVES of them
     int nsplit;                              // pieces that the bank's rows are cut into
     float c2;                                // scale * log2(e)
     float *part;                             // nsplit > 1: [split][batch heads][R][W] partial sums ...

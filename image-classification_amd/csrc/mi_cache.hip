@@ -1,4 +1,5 @@
 // mi_cache.hip -- C ABI (include/mi_knn.h) of the 4-bit cache bank: argument checks, launch shapes, workspaces.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -26,7 +27,7 @@ int check_cache(const mi_cache_t *c, const char *who)
         return fail(MI_ERR_ARG, "%s: null pointer in the cache", who);
     if (((uintptr_t)c->key | (uintptr_t)c->key_scale | (uintptr_t)c->value | (uintptr_t)c->value_scale | (uintptr_t)c->weight | (uintptr_t)c->position) & 15)
         return fail(MI_ERR_ARG, "%s: the cache's buffers must be 16-byte aligned", who);
-    if (c->batch < 1 || c->heads < 1 || c->batch * c->heads > (1 << 24) || c->batch > (1 << 24) || c->heads > (1 << 24))
+    if (c->batch < 1 || c->heads < 1 || c->batch > (1 << 24) || c->heads > (1 << 24) || c->batch * c->heads > (1 << 24))
         return fail(MI_ERR_ARG, "%s: bad shape batch=%lld heads=%lld", who, (long long)c->batch, (long long)c->heads);
     if (!width_of(c->dim)) return fail(MI_ERR_UNSUPPORTED, "%s: dim=%lld must be a multiple of 8 in [8, 256]", who, (long long)c->dim);
     if (c->limit < 1 || c->rows < c->limit || c->rows % 64 || c->rows > MAX_ROWS)
@@ -296,7 +297,8 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     MI_TRY(check_cache(cache, "mi_cache_attend"));
     if (!known_dtype(dtype)) return fail(MI_ERR_ARG, "mi_cache_attend: unknown dtype %d", dtype);
     if (T < 0 || group < 1 || group > 65536 || T > MAX_ROWS / group) return fail(MI_ERR_ARG, "mi_cache_attend: bad shape T=%lld group=%lld", (long long)T, (long long)group);
-    if (!(scale > 0.f) || !isfinite(scale)) return fail(MI_ERR_ARG, "mi_cache_attend: scale must be positive and finite");
+    // a scale that the base 2 exponent cannot hold would make NaN of masked scores
+    if (!(scale * mi::CACHE_LOG2E >= FLT_MIN) || !isfinite(scale * mi::CACHE_LOG2E)) return fail(MI_ERR_ARG, "mi_cache_attend: scale must be positive and finite, got %g", (double)scale);
     if (T == 0) return MI_OK;
     mi::CacheAttendParams p{};
     MI_TRY(check_rows("mi_cache_attend", "query", query, query_strides, dtype, p.q_s));

@@ -131,7 +131,7 @@ def test_abi_refuses_bad_calls_before_touching_the_device():
     def attend(scale=1.0, ws=at, nbytes=1 << 30, group=1, T=1, dtype=1, out=at):
         return L.mi_cache_attend(cache(), at, s, out, s, dtype, T, group, None, scale, 1, 0, 10, ws, nbytes, None)
 
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 3e38, 1e-39):
         assert attend(scale=scale) == -1 and b"scale" in L.mi_last_error()
     assert attend(ws=None) == -1 and attend(nbytes=1) == -3 and attend(group=0) == -1 and attend(T=-1) == -1 and attend(dtype=3) == -1 and attend(out=None) == -1
     assert L.mi_cache_attend_workspace_bytes(cache(), 1, 0, 1, 10, 1, 0) == 0 and L.mi_cache_attend_workspace_bytes(cache(), 9, 1, 1, 10, 1, 0) == 0
