@@ -67,6 +67,13 @@ def _aligned(t: torch.Tensor):
     return t, _strides(t)
 
 
+def _part_shapes(k, batch, heads, dim):
+    width = 64 if dim <= 64 else 128 if dim <= 128 else 256
+    rows = (k + 63) // 64 * 64
+    held, scales, each = (batch, heads, rows, width // 2), (batch, heads, width // 32, rows), (batch, heads, rows)
+    return held, scales, held, scales, each, each, (batch,), (batch,)
+
+
 class CacheBank(nn.Module):
     """Named 4-bit banks of keys and values: ``register``, ``push``, ``attend``, ``evict``, ``trim``, ``bank[name]``."""
 
@@ -76,7 +83,7 @@ class CacheBank(nn.Module):
         self.shapes = {}           # name -> (batch, heads, dim)
         self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows
         self._captured = set()     # names whose lengths a graph may change behind the host's back
-        self._views = {}           # name -> (buffers, mi_cache_t over them, how to pick them)
+        self._views = {}           # name -> (buffers, mi_cache_t over them, how to pick them, where they start)
 
     def __getstate__(self):
         return {**self.__dict__, "_views": {}}
@@ -95,10 +102,7 @@ class CacheBank(nn.Module):
             raise ValueError(f"dim must be a multiple of 8 in [8, 256], got {dim}")
         if k < 1 or heads < 1 or batch < 1:
             raise ValueError(f"k, heads and batch must be positive, got k={k} heads={heads} batch={batch}")
-        width = 64 if dim <= 64 else 128 if dim <= 128 else 256
-        rows = (k + 63) // 64 * 64
-        held, scales = (batch, heads, rows, width // 2), (batch, heads, width // 32, rows)
-        for part, dtype, shape in zip(_PARTS, _DTYPES, (held, scales, held, scales, (batch, heads, rows), (batch, heads, rows), (batch,), (batch,))):
+        for part, dtype, shape in zip(_PARTS, _DTYPES, _part_shapes(k, batch, heads, dim)):
             self.register_buffer(f"{name}_{part}", torch.zeros(shape, dtype=dtype, device=device))
         self.sizes[name], self.shapes[name], self._bounds[name] = k, (batch, heads, dim), 0
         self._captured.discard(name)
@@ -109,20 +113,25 @@ class CacheBank(nn.Module):
         if name not in self.sizes:
             raise KeyError(f"CacheBank.{what}: no bank named {name!r}")
         known = self._views.get(name)
-        if known is not None and all(map(operator.is_, known[0], known[2](self._buffers))):
+        if known is not None and all(map(operator.is_, known[0], known[2](self._buffers))) and known[3] == [*map(torch.Tensor.data_ptr, known[0])]:
             return known[1], known[0]
         pick = operator.itemgetter(*[f"{name}_{part}" for part in _PARTS])
         held = pick(self._buffers)
         if not held[0].is_cuda:
             raise RuntimeError(f"CacheBank.{what}: buffer is on {held[0].device}; image-classification_amd moves bank rows "
                                "with HIP kernels only (no CPU fallback) -- call .to(device) first")
-        for part, dtype, t in zip(_PARTS, _DTYPES, held):
+        batch, heads, dim = self.shapes[name]
+        for part, dtype, shape, t in zip(_PARTS, _DTYPES, _part_shapes(self.sizes[name], batch, heads, dim), held):
+            if t.shape != shape:
+                raise RuntimeError(f"CacheBank.{what}: buffer {name}_{part} is {tuple(t.shape)}, the bank was registered with {shape}")
             if t.dtype != dtype or not t.is_contiguous() or t.device != held[0].device:
                 raise RuntimeError(f"CacheBank.{what}: buffer {name}_{part} must be contiguous {dtype} on {held[0].device}, "
                                    f"got {t.dtype} on {t.device} (move banks with .to(device), not to another dtype)")
-        batch, heads, dim = self.shapes[name]
-        view = ctypes.pointer(_lib.Cache(*[t.data_ptr() for t in held], batch, heads, dim, held[4].shape[2], self.sizes[name]))
-        self._views[name] = (held, view, pick)
+        starts = [t.data_ptr() for t in held]
+        view = ctypes.pointer(_lib.Cache(*starts, batch, heads, dim, held[4].shape[2], self.sizes[name]))
+        if known is not None:                      # other buffers than before, and other lengths for all the host knows
+            self._bounds[name] = self.sizes[name]
+        self._views[name] = (held, view, pick, starts)
         return view, held
 
     @staticmethod

@@ -604,3 +604,25 @@ def test_other_streams_state_dicts_and_copies():
     other.trim("kv")
     assert torch.equal(bank.attend("kv", q), want) and not other.attend("kv", q).any()
     _rows_equal(bank, ref)
+
+
+@gpu
+def test_buffers_that_were_replaced():
+    rs = np.random.RandomState(11)
+    bank, ref = _filled(rs, 2, 1, 64, 64, 50)
+    q = _rand(rs, (2, 1, 2, 64), "bf16", 0.3).cuda()
+    want = bank.attend("kv", q)
+    for part in ("key", "value", "length"):                                             # the same tensors over other memory
+        old = bank._buffers[f"kv_{part}"].data
+        bank._buffers[f"kv_{part}"].data = old.clone()
+        old.zero_()
+    assert torch.equal(bank.attend("kv", q), want)
+    _rows_equal(bank, ref)
+    bank.trim("kv", 10)
+    bank.kv_length = torch.full((2,), 60, dtype=torch.int32, device="cuda")
+    z = torch.zeros(2, 1, 5, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="do not fit"):
+        bank.push("kv", z, z)
+    bank.kv_weight = bank.kv_weight[:1].clone()
+    with pytest.raises(RuntimeError, match="kv_weight"):
+        bank.attend("kv", q)
