@@ -337,6 +337,7 @@ struct CacheAttendParams {
     int T, G, causal;                        // G query heads read one head of the bank
     int R, tiles;                            // R = T G rows per (sequence, head), row = t G + g; tiles of 16 MT or 32 WAVES of them
     int nsplit;                              // pieces that the bank's rows are cut into
+    int mixed;                               // tiled form: pieces in another order for each tile
     float c2;                                // scale * log2(e)
     float *part;                             // nsplit > 1: [split][batch heads][R][W] partial sums ...
     float2 *part_ml;                         //             ... and [split][batch heads][R] (maximum, sum), maximum in log2 units
@@ -830,10 +831,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
     constexpr int RING = 4;                  // operands on their way: read right before its use, one waits for shared memory longer than for the matrix core
     extern __shared__ uint4 s_tile[];        // [2][KF + VF][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, l = lane >> 5;
-    // heads innermost (a head's bank stays in one die's cache where heads are a multiple of 8), the longest rows first
+    // Heads innermost (a head's bank stays in one die's cache where heads are a multiple of 8), the longest rows first.  Workgroups
+    // go to the eight dies in turn: where pieces differ in length (the first one of causal rows is the longest), their order changes
+    // with the tile, by a number whose parity no die has one of; an even number of them would leave half of the dies the long ones.
     const int bhs = p.c.batch * p.c.heads;
     const long long bh = blockIdx.x % bhs;
-    const int rest = (int)(blockIdx.x / bhs), split = rest % p.nsplit, tile = p.tiles - 1 - rest / p.nsplit;
+    const int rest = (int)(blockIdx.x / bhs), turn = rest / p.nsplit, tile = p.tiles - 1 - turn;
+    const int split = (rest % p.nsplit + (p.mixed ? __popc(turn) : 0)) % p.nsplit;
     const int b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads);
     const int len = rows_used(p.c, b);
     const int n = real_rows(p.counts, b, p.T);

@@ -74,24 +74,33 @@ struct AttendPlan {
     int64_t R, mt, tiles, nsplit;
     bool tiled;                              // 32 `waves` query rows a workgroup through shared memory, not 16 mt straight from memory
     int waves;
+    bool uneven;                             // tiled, causal, mostly its own rows: the first pieces are longer than the last
     int64_t chunks, rsplit;                  // weights: workgroups a (sequence, head) along the bank, and along the query rows
     bool scores;                             // weights: from scores left behind, not from a second product
     size_t off_ml, off_norm, off_scores, off_w, total;
 };
 
-// How long the tiled form takes, in tiles of 128 rows of the bank by 256 query rows on one compute unit, with `waves` waves a
-// workgroup and the bank in `nsplit` pieces: the larger of an even share and the longest piece where pieces differ (causal, mostly
-// its own rows), whole rounds of equal pieces otherwise.  Measured: a workgroup of four waves (two a unit) needs 1 / 0.9 of the time
-// of one of eight for the same work; a tile is 3.8 us; getting started and leaving costs about 1.3 of them; joining pieces one, and
-// the writing and reading of their sums.
-double tiled_cost(int64_t bh, int64_t R, int width, int64_t span, double seen, bool uneven, int waves, int64_t nsplit)
+// How long the tiled form takes, in tiles of 128 rows of the bank by 256 query rows, bf16 and 128 dims, on one compute unit (3.8 us),
+// with `waves` waves a workgroup and the bank in `nsplit` pieces: the larger of an even share and the longest piece where pieces
+// differ (causal, mostly its own rows), whole rounds of equal pieces otherwise.  Measured: other widths and types cost `work`
+// (1.2 us a step of a workgroup of four waves at bf16 and 128 dims, 2.0 at 256, 1.9 / 2.5 for fp16 / fp32, 1.6 for fp32 at 64); four
+// waves need 0.31 for a quarter of a tile alone on a unit, 0.2775 beside another workgroup, which fp32 and 256 dims leave no room for;
+// getting started and leaving costs about 1.3; joining pieces one, and the writing and reading of their sums.
+double tiled_cost(int64_t bh, int64_t R, int width, int dtype, int64_t span, double seen, bool uneven, int waves, int64_t nsplit)
 {
-    const int64_t tiles = ceil_div(R, 32 * waves), units = ceil_div(span, 16 * waves), per = ceil_div(units, nsplit);
-    const double slots = waves == 8 ? 256 : 512, unit = waves == 8 ? 1.0 : 0.5 / 0.9, over = 1.3;
+    const int64_t tiles = ceil_div(R, 32 * waves), units = ceil_div(span, 16 * waves), per = ceil_div(units, nsplit), all = bh * tiles * nsplit;
+    const bool pairs = waves == 4 && dtype != MI_F32 && width < 256;
+    const double pieces = dtype == MI_BF16 ? 1 : dtype == MI_F16 ? 2 : 3, work = 0.37 + 0.63 * width / 128 * pieces;
+    const double alone = (waves == 8 ? 1.0 : 0.31) * work, busy = pairs ? 0.2775 * work : alone, over = 1.3;
     const double share = seen / (double)span, groups = (double)(bh * tiles);
+    const int64_t slots = pairs ? 512 : 256, turns = ceil_div(all, 256);
     double t;
-    if (uneven) t = std::max(groups * ((double)units * share * unit + over * std::max(1.0, (double)nsplit * share)) / slots, (double)per * unit * (waves == 8 ? 1.0 : 0.8) + over);
-    else t = ceil(groups * (double)nsplit / slots) * ((double)per * unit + over);
+    if (uneven) {
+        const bool few = groups * ((double)nsplit * share + 0.5) <= 288;      // workgroups that have anything to do: hardly two on a unit
+        t = std::max(groups * ((double)units * share * busy / 256 + over * std::max(1.0, (double)nsplit * share) / (double)slots),
+                     (double)per * (few ? alone : pairs ? 1.6 * busy : busy) + over);
+    }
+    else t = (double)(turns * per) * (turns == 1 ? alone : busy) + (double)ceil_div(all, slots) * over;
     return t + (nsplit > 1 ? 1.0 + (double)(bh * R * nsplit) * width * 8 / (4.5e12 * 3.8e-6) : 0.0);
 }
 
@@ -106,10 +115,11 @@ AttendPlan attend_plan(const mi_cache_t *c, int dtype, int64_t T, int64_t group,
     if (a.tiled) {
         const double seen = causal ? std::max((double)span * 0.5, (double)span - (double)T * 0.5) : (double)span;
         const int64_t most = std::min<int64_t>(ceil_div(span, 256), mi::CACHE_MAX_SPLIT);
+        a.uneven = causal && 2 * T > span;
         double best = 1e300;
         for (int waves = dtype == MI_BF16 && width_of(c->dim) < 256 ? 8 : 4; waves >= 4; waves -= 4)
             for (int64_t ns = 1; ns <= most; ++ns) {
-                const double t = tiled_cost(bh, a.R, width_of(c->dim), span, seen, causal && 2 * T > span, waves, ns);
+                const double t = tiled_cost(bh, a.R, width_of(c->dim), dtype, span, seen, a.uneven, waves, ns);
                 if (t < best) best = t, a.waves = waves, a.nsplit = ns;
             }
         a.tiles = ceil_div(a.R, 32 * a.waves);
@@ -316,7 +326,7 @@ int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *q
     p.out = (char *)out;
     p.counts = counts;
     p.T = (int)T, p.G = (int)group, p.causal = causal ? 1 : 0;
-    p.R = (int)a.R, p.tiles = (int)a.tiles, p.nsplit = (int)a.nsplit, p.chunks = (int)a.chunks;
+    p.R = (int)a.R, p.tiles = (int)a.tiles, p.nsplit = (int)a.nsplit, p.mixed = a.uneven, p.chunks = (int)a.chunks;
     p.c2 = scale * mi::CACHE_LOG2E;
     p.part = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + a.off_ml);

@@ -292,6 +292,27 @@ def test_attend_against_64_bits(dtype, dim, H, group, T, fill):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim,H,group,T,fill", [(64, 1, 1, 1100, 1150), (128, 1, 2, 1000, 1000), (256, 2, 1, 777, 1290), (128, 2, 1, 1025, 2000)])
+def test_attend_causal_prompts_in_pieces(dtype, dim, H, group, T, fill):
+    """Few heads and mostly their own rows: the bank is cut into pieces whose order changes with the tile; most rows see only some of
+    them, and those of the shorter sequences (less than T rows) nothing at all at first."""
+    rs = np.random.RandomState(T)
+    bank, ref = _filled(rs, 2, H, dim, fill, fill)
+    q = _rand(rs, (2, H * group, T, dim), dtype, 0.3)
+    for counts in (None, [T - 1, T // 3]):
+        out = bank.attend("kv", q.cuda(), counts=counts, accumulate=True)
+        want = ref.attend(_np(q), counts, accumulate=True)
+        _check_out(out, want[0], want[1], dtype, T * group)
+        for b in range(2):
+            for h in range(H):
+                n = ref.length(b)
+                d = np.abs(_np(bank.weights("kv"))[b, h, :n] - ref.weight[b][h])
+                assert (d <= want[2][b][h] + 1e-12).all(), d.max()
+                ref.weight[b][h] = _np(bank.weights("kv"))[b, h, :n]
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_attend_large_scores_and_other_scales(dtype):
     """Scores of several hundred: one row takes all, in a far corner of the bank, and the running maximum moves late."""
