@@ -161,7 +161,13 @@ def main():
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
     if not torch.cuda.is_available():
-        raise SystemExit("bench.py needs an MI355X: torch.cuda.is_available() is False")
+        text = "bench.py needs an MI355X: torch.cuda.is_available() is False"
+        if world > 1:
+            # a launcher ends the other ranks as soon as one has failed: each gets the time to say the same
+            print(text, file=sys.stderr, flush=True)
+            time.sleep(3)
+            raise SystemExit(1)
+        raise SystemExit(text)
     dev_index = 0 if args.rehearse_shared_gpu else local_rank
     torch.cuda.set_device(dev_index)
     device = torch.device("cuda", dev_index)
