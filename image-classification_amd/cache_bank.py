@@ -283,7 +283,8 @@ class CacheBank(nn.Module):
 
     def trim(self, name, lengths=0):
         """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
-        the bank, a smaller length takes back the rows pushed last (a rejected draft).  Positions go on from the cut."""
+        the bank, a smaller length takes back the rows pushed last (a rejected draft), by position, wherever an eviction has put them:
+        freed slots below the new length take, in ascending order, the rows that stay from above.  Positions go on from the cut."""
         view, held_by = self._cache(name, "trim")
         device = held_by[0].device
         each, number = None, 0

@@ -266,17 +266,140 @@ __global__ __launch_bounds__(256) void cache_longest_kernel(PushParams p, int *o
     if (threadIdx.x == 0) *out = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
 }
 
-// Every sequence is cut to at most its entry of `lengths` (or `length`); positions go on from where the cut left them.
-__global__ void cache_trim_kernel(CacheView c, const int *lengths, int length)
+// Every sequence is cut to at most its entry of `lengths` (or `length`): of each head the rows pushed last leave.  Where no row of the
+// sequence was ever evicted, or what leaves lies behind the new length in the order of its pushes, that is all there is to do.  An
+// eviction puts rows from above into freed slots, so that a row's slot says nothing of its age: then the rows with the largest positions
+// leave, and the slots that they free below the new length take the rows that stay from above it, both in ascending order (as an
+// eviction does; no row is read that another one is written to).  Positions go on from the cut, and in any case behind all that stay.
+// One workgroup a sequence: the order is looked at in 4 bytes a head and row that leaves; only a cut that finds rows out of order
+// goes over a bank, head by head.
+constexpr int TRIM_THREADS = 1024;
+
+struct TrimShared {
+    int hist[256], wave[TRIM_THREADS / 64];
+    int holes[2 * TRIM_THREADS], tails[TRIM_THREADS];
+    int pick[3], out_of_order, last;
+};
+
+// How many threads before this one have `mine` set, and how many have it in all.
+__device__ __forceinline__ int block_rank(bool mine, TrimShared &sh, int &all)
 {
-    const int b = blockIdx.x * 64 + threadIdx.x;
-    if (b >= c.batch) return;
+    const unsigned long long who = __ballot(mine);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (lane == 0) sh.wave[wave] = __popcll(who);
+    __syncthreads();
+    int before = __popcll(who & ((1ull << lane) - 1));
+    all = 0;
+    for (int i = 0; i < TRIM_THREADS / 64; ++i) {
+        if (i < wave) before += sh.wave[i];
+        all += sh.wave[i];
+    }
+    return before;
+}
+
+// Lets the `gone` youngest of the `len` rows of one head leave and puts the others into slots 0 .. n = len - gone.
+__device__ __forceinline__ void trim_head(const CacheView &c, long long bh, int width, int len, int n, TrimShared &sh)
+{
+    const int tid = threadIdx.x;
+    int *const pos = c.position + bh * c.rows;
+    const auto age = [&](int slot) { return (uint32_t)pos[slot] ^ 0x80000000u; };      // in the order of the positions
+    // the position that the gone-th youngest row has, by digits of 8 bits from the top; `left` of the rows on it leave, the highest slots
+    uint32_t edge = 0;
+    int left = len - n, ties = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += TRIM_THREADS) sh.hist[i] = 0;
+        __syncthreads();
+        const uint32_t known = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+        for (int i = tid; i < len; i += TRIM_THREADS) {
+            const uint32_t u = age(i);
+            if ((u & known) == edge) atomicAdd(&sh.hist[u >> shift & 255u], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int digit = 255, rest = left;
+            while (digit > 0 && sh.hist[digit] < rest) rest -= sh.hist[digit--];
+            sh.pick[0] = digit, sh.pick[1] = rest, sh.pick[2] = sh.hist[digit];
+        }
+        __syncthreads();
+        edge |= (uint32_t)sh.pick[0] << shift;
+        left = sh.pick[1];
+        ties = sh.pick[2];
+        __syncthreads();
+    }
+    const int tied = ties - left;            // rows on the edge that stay: the lowest slots
+    // whether a row leaves, asked for TRIM_THREADS neighbours at a time in ascending order; `on` counts the rows on the edge so far
+    const auto leaves = [&](int slot, int end, int &on) {
+        const uint32_t u = slot < end ? age(slot) : 0u;
+        int all;
+        const int before = on + block_rank(slot < end && u == edge, sh, all);
+        on += all;
+        return slot < end && (u > edge || (u == edge && before >= tied));
+    };
+    int on_hole = 0, on_tail = 0, all;
+    for (int i0 = 0; i0 < n; i0 += TRIM_THREADS) {
+        block_rank(i0 + tid < n && age(i0 + tid) == edge, sh, all);
+        on_tail += all;
+    }
+    const int words = width / 32, parts = 4 * words + 2;          // 16 bytes of key or value, or a byte of their scales, for each 32 dims
+    int found = 0, filled = 0, hole0 = 0;    // freed slots found, and taken; where the search goes on
+    for (int t0 = n; t0 < len; t0 += TRIM_THREADS) {
+        const bool stays = t0 + tid < len, gone = leaves(t0 + tid, len, on_tail);
+        const int at = block_rank(stays && !gone, sh, all);
+        const int tails = all;
+        if (stays && !gone) sh.tails[at] = t0 + tid;
+        while (found < filled + tails && hole0 < n) {             // as many freed slots as rows that stay: at most 2 TRIM_THREADS wait
+            const bool hole = leaves(hole0 + tid, n, on_hole);
+            const int k = block_rank(hole, sh, all);
+            if (hole) sh.holes[(found + k) % (2 * TRIM_THREADS)] = hole0 + tid;
+            found += all;
+            hole0 += TRIM_THREADS;
+        }
+        __syncthreads();
+        const int moves = min(tails, found - filled);
+        for (int i = tid; i < moves * parts; i += TRIM_THREADS) {
+            const int k = i / parts, part = i - k * parts, src = sh.tails[k], dst = sh.holes[(filled + k) % (2 * TRIM_THREADS)];
+            if (part < 2 * words) {
+                uint8_t *side = (part < words ? c.key : c.value) + bh * c.rows * (width / 2) + part % words * 16;
+                *(uint4 *)(side + (long long)dst * (width / 2)) = *(const uint4 *)(side + (long long)src * (width / 2));
+            } else if (part < 4 * words) {
+                uint8_t *side = (part < 3 * words ? c.key_scale : c.value_scale) + (bh * words + part % words) * c.rows;
+                side[dst] = side[src];
+            } else if (part == 4 * words) c.weight[bh * c.rows + dst] = c.weight[bh * c.rows + src];
+            else pos[dst] = pos[src];
+        }
+        filled += moves;
+        __syncthreads();
+    }
+    int last = -1;                           // of the rows that stay
+    for (int i = tid; i < n; i += TRIM_THREADS) last = max(last, pos[i]);
+    atomicMax(&sh.last, last);
+}
+
+__global__ __launch_bounds__(TRIM_THREADS) void cache_trim_kernel(CacheView c, const int *lengths, int length, int width)
+{
+    __shared__ TrimShared sh;
+    const int b = blockIdx.x, tid = threadIdx.x;
     int n = lengths ? lengths[b] : length;
     n = n < 0 ? 0 : n;
-    const int gone = rows_used(c, b) - n;
-    if (gone > 0) {
+    const int len = rows_used(c, b), gone = len - n, seen = c.seen[b];
+    if (gone <= 0) return;
+    if (tid == 0) sh.out_of_order = 0, sh.last = -1;
+    __syncthreads();
+    if (n > 0 && seen != len) {
+        const long long all = (long long)c.heads * gone;
+        for (long long i = tid; i < all; i += TRIM_THREADS) {
+            const int h = (int)(i / gone), slot = n + (int)(i - (long long)h * gone);
+            if (c.position[((long long)b * c.heads + h) * c.rows + slot] != seen - len + slot) sh.out_of_order = 1;
+        }
+        __syncthreads();
+        if (sh.out_of_order)
+            for (int h = 0; h < c.heads; ++h) trim_head(c, (long long)b * c.heads + h, width, len, n, sh);
+    }
+    __syncthreads();
+    if (tid == 0) {
         c.length[b] = n;
-        c.seen[b] -= gone;
+        c.seen[b] = max(seen - gone, sh.last + 1);
     }
 }
 

@@ -272,7 +272,8 @@ int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t lengt
 {
     MI_TRY(check_cache(cache, "mi_cache_trim"));
     if (!lengths && (length < 0 || length > INT32_MAX)) return fail(MI_ERR_ARG, "mi_cache_trim: bad length %lld", (long long)length);
-    hipLaunchKernelGGL(mi::cache_trim_kernel, dim3((unsigned)ceil_div(cache->batch, 64)), dim3(64), 0, (hipStream_t)stream, view(cache), lengths, (int)length);
+    hipLaunchKernelGGL(mi::cache_trim_kernel, dim3((unsigned)cache->batch), dim3(mi::TRIM_THREADS), 0, (hipStream_t)stream, view(cache), lengths, (int)length,
+                       width_of(cache->dim));
     HIP_CHECK(hipGetLastError());
     return MI_OK;
 }

@@ -258,7 +258,10 @@ int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_s
 /* *out (device) = the most rows that a sequence would have after mi_cache_push of these counts, whether they fit or not. */
 int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream);
 
-/* length[b] = min(length[b], lengths[b]) (device int32[batch]; NULL: `length` for all); positions go on from the cut. */
+/* length[b] = min(length[b], lengths[b]) (device int32[batch]; NULL: `length` for all): of each head the rows pushed last leave, by
+ * position.  Where an eviction has left them in slots below the new length, these take, in ascending order, the rows that stay of the
+ * slots above.  Positions go on from the cut, and behind every row that stays (a head that evicted some of the rows pushed last loses
+ * older ones instead).  Attention sums that query rows have left on other rows stay. */
 int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t length, mi_stream_t stream);
 
 /* Rows [0, limit) as bf16 (exact), [batch][heads][limit][dim] each; rows that are not in use are zeros. */
