@@ -15,8 +15,10 @@ layouts and the number format in ``include/mi_knn.h``), so ``.to(device)`` and `
 its own sequences: nothing is gathered.  No gradients: the bank is memory, as the MoCo queue is.  No CPU path.
 
 Lengths live on the device and no call waits for it, except a ``push`` that may run over: the host knows an upper bound of the lengths and
-reads them back when that bound plus the new rows passes ``k``.  All calls can be captured into a graph; a captured ``push`` cannot look,
-and rows that do not fit when it is replayed are dropped."""
+reads them back when that bound plus the new rows passes ``k``, or when torch has written to the lengths, or put others in their place,
+since it knew it.  (A collective or a kernel of one's own that writes to them in place goes unnoticed: load them with ``load_state_dict``
+or ``copy_``.)  All calls can be captured into a graph; a captured ``push`` cannot look, and rows that do not fit when it is replayed are
+dropped."""
 from __future__ import annotations
 
 import contextlib
@@ -67,6 +69,12 @@ def _aligned(t: torch.Tensor):
     return t, _strides(t)
 
 
+def _mark(t: torch.Tensor):
+    """Tells whether torch has written to ``t``, or it has come to lie elsewhere, since an earlier mark that this one equals.  Writes to an
+    inference tensor are not counted: no two of its marks are equal."""
+    return t.data_ptr(), object() if t.is_inference() else t._version
+
+
 def _part_shapes(k, batch, heads, dim):
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     rows = (k + 63) // 64 * 64
@@ -81,12 +89,13 @@ class CacheBank(nn.Module):
         super().__init__()
         self.sizes = {}            # name -> k
         self.shapes = {}           # name -> (batch, heads, dim)
-        self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows
+        self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows ...
+        self._marks = {}           # name -> ... and the lengths that this was said of: (buffer, its mark)
         self._captured = set()     # names whose lengths a graph may change behind the host's back
         self._views = {}           # name -> (buffers, mi_cache_t over them, how to pick them, where they start)
 
     def __getstate__(self):
-        return {**self.__dict__, "_views": {}}
+        return {**self.__dict__, "_views": {}, "_marks": {}}
 
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
@@ -104,8 +113,9 @@ class CacheBank(nn.Module):
             raise ValueError(f"k, heads and batch must be positive, got k={k} heads={heads} batch={batch}")
         for part, dtype, shape in zip(_PARTS, _DTYPES, _part_shapes(k, batch, heads, dim)):
             self.register_buffer(f"{name}_{part}", torch.zeros(shape, dtype=dtype, device=device))
-        self.sizes[name], self.shapes[name], self._bounds[name] = k, (batch, heads, dim), 0
+        self.sizes[name], self.shapes[name] = k, (batch, heads, dim)
         self._captured.discard(name)
+        self._set_bound(name, 0)
         self._views.pop(name, None)
 
     # ------------------------------------------------------------------------------------------------------------ helpers
@@ -129,8 +139,7 @@ class CacheBank(nn.Module):
                                    f"got {t.dtype} on {t.device} (move banks with .to(device), not to another dtype)")
         starts = [t.data_ptr() for t in held]
         view = ctypes.pointer(_lib.Cache(*starts, batch, heads, dim, held[4].shape[2], self.sizes[name]))
-        if known is not None:                      # other buffers than before, and other lengths for all the host knows
-            self._bounds[name] = self.sizes[name]
+        self._bound(name)
         self._views[name] = (held, view, pick, starts)
         return view, held
 
@@ -169,7 +178,16 @@ class CacheBank(nn.Module):
             return True
         return False
 
+    def _bound(self, name) -> int:
+        """The bound, where it still speaks of the lengths that the bank has; otherwise they may be anything up to ``k``."""
+        held, length = self._marks.get(name, (None, None)), self._buffers[f"{name}_length"]
+        if held[0] is not length or held[1] != _mark(length):
+            self._set_bound(name, self.sizes[name])
+        return self._bounds[name]
+
     def _set_bound(self, name, bound):
+        length = self._buffers[f"{name}_length"]
+        self._marks[name] = length, _mark(length)
         self._bounds[name] = self.sizes[name] if name in self._captured else min(bound, self.sizes[name])
 
     def _span(self, name) -> int:
@@ -195,7 +213,7 @@ class CacheBank(nn.Module):
         counts = self._counts(counts, key.shape[0], T, device)
         with _on(device):
             if not self._changes(name):
-                bound = k if name in self._captured else self._bounds[name]
+                bound = k if name in self._captured else self._bound(name)
                 if bound + T > k:                       # the one place that waits for the device
                     longest = torch.empty(1, dtype=torch.int32, device=device)
                     _lib.check(_lib.lib().mi_cache_longest(view, None if counts is None else counts.data_ptr(), T, longest.data_ptr(),
@@ -279,7 +297,7 @@ class CacheBank(nn.Module):
             span = self._span(name)
             _lib.check(L.mi_cache_evict(view, other, keep, recent, span, ws.data_ptr(), ws.numel(),
                                         _lib.raw_stream(device.index)), "mi_cache_evict")
-        self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bounds[name]))
+        self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bound(name)))
 
     def trim(self, name, lengths=0):
         """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
@@ -300,7 +318,8 @@ class CacheBank(nn.Module):
             self._changes(name)
             _lib.check(_lib.lib().mi_cache_trim(view, None if each is None else each.data_ptr(), number,
                                                 _lib.raw_stream(device.index)), "mi_cache_trim")
-        self._set_bound(name, self._bounds[name] if each is not None else min(number, self._bounds[name]))
+        bound = self._bound(name)
+        self._set_bound(name, bound if each is not None else min(number, bound))
 
     def __getitem__(self, name):
         """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""

@@ -170,3 +170,71 @@ def test_trim_in_a_graph_goes_by_age():
         _rows_equal(bank, ref)
         _weights_equal(bank, ref)
         _push(bank, ref, rs, 20)                                                         # eager work between the replays
+
+
+# ----------------------------------------------------------------------------------------------- buffers changed from outside
+def _full(bank, value, part="length"):
+    return torch.full((bank.shapes["kv"][0],), value, dtype=torch.int32, device="cuda")
+
+
+@gpu
+@pytest.mark.parametrize("how", ["before the first call", "in place", "through a view", "other memory", "after a copy", "after a pickle", "inference"])
+def test_push_notices_lengths_that_were_changed(how):
+    """Whatever torch wrote to a bank's lengths, before its first call, between calls or in a copy of it: a push that does not fit is refused."""
+    import pickle
+    bank = _ica().CacheBank()
+    if how == "inference":
+        with torch.inference_mode():
+            bank.register("kv", dim=64, k=64, batch=2)
+    else:
+        bank.register("kv", dim=64, k=64, batch=2)
+    z = torch.zeros(2, 1, 5, 64, device="cuda")
+    if how not in ("before the first call",):
+        bank.push("kv", z, z)
+    if how == "after a copy":
+        bank = copy.deepcopy(bank)
+    if how == "after a pickle":
+        bank = pickle.loads(pickle.dumps(bank))
+    if how in ("in place", "inference"):
+        with torch.inference_mode(how == "inference"):
+            bank.lengths("kv").fill_(60)
+    elif how == "through a view":
+        bank.state_dict()["kv_length"][1:].add_(55)
+    elif how == "other memory":
+        bank._buffers["kv_length"].data = _full(bank, 60)
+    else:
+        bank.kv_length = _full(bank, 60)
+    before = bank.lengths("kv").tolist()
+    with pytest.raises(RuntimeError, match="do not fit"):
+        bank.push("kv", z, z)
+    assert bank.lengths("kv").tolist() == before
+    bank.push("kv", z[:, :, :4], z[:, :, :4])
+    assert max(bank.lengths("kv").tolist()) == 64
+    with pytest.raises(RuntimeError, match="do not fit"):
+        bank.push("kv", z[:, :, :1], z[:, :, :1])
+
+
+@gpu
+def test_push_does_not_look_where_lengths_are_known():
+    bank = _ica().CacheBank()
+    bank.register("kv", dim=64, k=64, batch=2)
+    z = torch.zeros(2, 1, 8, 64, device="cuda")
+    L = _ica()._lib.lib()
+    real, looks = L.mi_cache_longest, []
+    L.mi_cache_longest = lambda *a: looks.append(1) or real(*a)
+    try:
+        for _ in range(8):
+            bank.push("kv", z, z)
+        bank.evict("kv", 40)
+        bank.push("kv", z, z)
+        bank.trim("kv", 10)
+        bank.push("kv", z, z)
+        assert not looks
+        bank.lengths("kv").fill_(3)
+        bank.push("kv", z, z)
+        assert len(looks) == 1
+        for _ in range(5):
+            bank.push("kv", z, z)
+        assert len(looks) == 1 and bank.lengths("kv").tolist() == [51, 51]
+    finally:
+        L.mi_cache_longest = real
