@@ -12,13 +12,13 @@ LIB_PATH = os.environ.get("MI_KNN_LIB") or os.path.join(HERE, "libmi_knn.so")   
 
 MI_F32, MI_BF16, MI_F16 = 0, 1, 2
 MI_MAX_K, MI_MAX_CLASSES = 1024, 65536
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 EXPORTS = [
     "mi_abi_version", "mi_last_error", "mi_profile_enable", "mi_profile_collect", "mi_profile_clock", "mi_debug_force_fallback", "mi_knn_ld", "mi_pack_rows", "mi_knn_topk_workspace_bytes", "mi_knn_topk_workspace_bytes_for_budget",
     "mi_knn_topk", "mi_knn_topk_static", "mi_knn_merge", "mi_knn_vote", "mi_queue_push", "mi_bank_scatter", "mi_moco_workspace_bytes",
     "mi_moco_fwd", "mi_moco_bwd", "mi_queue_push_stash", "mi_bank_append_normalized", "mi_queue_push_wrap", "mi_soft_knn_workspace_bytes", "mi_soft_knn", "mi_kth_largest",
-    "mi_cache_width", "mi_cache_push", "mi_cache_longest", "mi_cache_trim", "mi_cache_read", "mi_cache_attend_workspace_bytes", "mi_cache_attend",
+    "mi_cache_width", "mi_cache_push", "mi_cache_longest", "mi_cache_in_order", "mi_cache_trim", "mi_cache_read", "mi_cache_attend_workspace_bytes", "mi_cache_attend",
     "mi_cache_evict_workspace_bytes", "mi_cache_evict",
 ]
 
@@ -95,6 +95,7 @@ def lib() -> ctypes.CDLL:
     L.mi_cache_push.restype = i32
     L.mi_cache_push.argtypes = [cache, p, strides, p, strides, i32, i64, p, p, p, p]
     L.mi_cache_longest.restype, L.mi_cache_longest.argtypes = i32, [cache, p, i64, p, p]
+    L.mi_cache_in_order.restype, L.mi_cache_in_order.argtypes = i32, [cache, p, i64, p, p]
     L.mi_cache_trim.restype, L.mi_cache_trim.argtypes = i32, [cache, p, i64, p]
     L.mi_cache_read.restype, L.mi_cache_read.argtypes = i32, [cache, p, p, p]
     L.mi_cache_attend_workspace_bytes.restype = sz

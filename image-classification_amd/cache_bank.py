@@ -91,7 +91,10 @@ class CacheBank(nn.Module):
         self.shapes = {}           # name -> (batch, heads, dim)
         self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows ...
         self._marks = {}           # name -> ... and the lengths that this was said of: (buffer, its mark)
+        self._pushed = {}          # name -> rows pushed since slots may have stopped telling a row's age, or None: they tell it
         self._captured = set()     # names whose lengths a graph may change behind the host's back
+        self._mixed = set()        # names whose rows a graph may put into another order
+        self._loaded = set()       # names whose rows came from elsewhere, in an order that the host has not seen
         self._views = {}           # name -> (buffers, mi_cache_t over them, how to pick them, where they start)
 
     def __getstate__(self):
@@ -99,7 +102,7 @@ class CacheBank(nn.Module):
 
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
-        self._bounds = dict(self.sizes)
+        self._bounds, self._pushed, self._loaded = dict(self.sizes), dict.fromkeys(self.sizes, 0), set(self.sizes)
 
     def register(self, name, dim, k, heads=1, batch=1, device=None):
         """An empty bank of ``k`` rows of ``dim`` values (a multiple of 8, at most 256) for each head of each sequence, on ``device``
@@ -115,6 +118,9 @@ class CacheBank(nn.Module):
             self.register_buffer(f"{name}_{part}", torch.zeros(shape, dtype=dtype, device=device))
         self.sizes[name], self.shapes[name] = k, (batch, heads, dim)
         self._captured.discard(name)
+        self._mixed.discard(name)
+        self._loaded.discard(name)
+        self._pushed[name] = None
         self._set_bound(name, 0)
         self._views.pop(name, None)
 
@@ -183,6 +189,9 @@ class CacheBank(nn.Module):
         held, length = self._marks.get(name, (None, None)), self._buffers[f"{name}_length"]
         if held[0] is not length or held[1] != _mark(length):
             self._set_bound(name, self.sizes[name])
+            if self._pushed[name] is None:
+                self._loaded.add(name)
+            self._pushed[name] = 0
         return self._bounds[name]
 
     def _set_bound(self, name, bound):
@@ -193,6 +202,39 @@ class CacheBank(nn.Module):
     def _span(self, name) -> int:
         """About how many rows are in use: what launches are sized by."""
         return max(1, self.sizes[name] if name in self._captured else self._bounds[name])
+
+    def _in_order(self, name, view, counts, T, device) -> bool:
+        """Whether the last T rows of every sequence (or ``counts`` of them) are the rows pushed last, in their order: waits for the device."""
+        order = torch.empty(1, dtype=torch.int32, device=device)
+        _lib.check(_lib.lib().mi_cache_in_order(view, None if counts is None else counts.data_ptr(), T, order.data_ptr(),
+                                                _lib.raw_stream(device.index)), "mi_cache_in_order")
+        return bool(order)
+
+    def _told(self, name):
+        """How many rows of the bank's end are in the order of their pushes: None for all, as far as the host knows."""
+        pushed = self._pushed[name]
+        return pushed if pushed is None and name not in self._mixed else 0 if name in self._captured else pushed
+
+    def _check_order(self, name, view, counts, T, device):
+        """Refuses causal attention of T rows where slots do not say which rows were pushed before which.  They do until rows are evicted,
+        and the rows pushed since then do; a look at the device says the same of others."""
+        told = self._told(name)
+        if told is None:
+            return
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            told = self._pushed[name]                                      # a graph's own pushes come before its attention
+        if told is None or T <= told:
+            return
+        text = (f"CacheBank.attend: the last rows of bank {name!r} are not the rows pushed last, in their order, since an evict moved rows: causal "
+                "attention of several rows comes after their push and before the next evict")
+        if capturing:
+            if name not in self._loaded:
+                raise RuntimeError(text + " (a graph cannot look; a call outside of it, before, can)")
+        elif self._in_order(name, view, None, T, device):
+            self._pushed[name] = T
+        elif counts is None or not self._in_order(name, view, counts, T, device):
+            raise RuntimeError(text)
 
     # --------------------------------------------------------------------------------------------------------------- calls
     def push(self, name, key, value, counts=None, held=False):
@@ -231,6 +273,8 @@ class CacheBank(nn.Module):
                                                 value.data_ptr(), _array(value_strides), _CODES[key.dtype], T,
                                                 None if counts is None else counts.data_ptr(), None if not held else out[0].data_ptr(),
                                                 None if not held else out[1].data_ptr(), _lib.raw_stream(device.index)), "mi_cache_push")
+            if self._pushed[name] is not None:
+                self._pushed[name] += T
         return out if held else None
 
     def attend(self, name, query, counts=None, scale=None, causal=True, accumulate=False):
@@ -238,9 +282,12 @@ class CacheBank(nn.Module):
         reads head ``h // group``.
 
         ``causal``: the query rows are the last rows of their sequence (push first, then attend), and row t does not see the rows after
-        its own; otherwise every row sees the whole sequence.  ``counts``: as in :meth:`push`, real rows of each sequence.  Rows that are not
-        real or see nothing give zeros.  ``scale``: positive, ``dim ** -0.5`` if not given.  ``accumulate`` adds to :meth:`weights` what
-        each row of the bank got, summed over query rows and the group's heads; :meth:`evict` goes by that."""
+        its own; otherwise every row sees the whole sequence.  An :meth:`evict` may put rows into other slots, which then do not say who came
+        before whom: causal attention of more than one row has to come before it, and is refused after it until as many rows are pushed
+        again, unless the last rows are still in their order (the host then waits for the device once, as it does for a state that was
+        loaded).  ``counts``: as in :meth:`push`, real rows of each sequence (after an eviction, the counts of the push).  Rows that are
+        not real or see nothing give zeros.  ``scale``: positive, ``dim ** -0.5`` if not given.  ``accumulate`` adds to :meth:`weights`
+        what each row of the bank got, summed over query rows and the group's heads; :meth:`evict` goes by that."""
         view, held_by = self._cache(name, "attend")
         device = held_by[0].device
         batch, heads, dim = self.shapes[name]
@@ -259,6 +306,8 @@ class CacheBank(nn.Module):
             out = torch.empty_like(query)
             if T == 0:
                 return out
+            if causal and T > 1:
+                self._check_order(name, view, counts, T, device)
             step, out_strides = 16 // out.element_size(), _strides(out)
             if out.stride(3) != 1 or out_strides[0] % step or out_strides[1] % step or out_strides[2] % step:
                 out = torch.empty(query.shape, dtype=query.dtype, device=device)
@@ -292,12 +341,22 @@ class CacheBank(nn.Module):
             raise ValueError(f"CacheBank.evict: recent={recent} outside [0, keep={keep}]")
         L = _lib.lib()
         with _on(device):
-            self._changes(target)
+            captured, bound = self._changes(target), self._bound(name)
             ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(view, keep)), dtype=torch.uint8, device=device)
             span = self._span(name)
             _lib.check(L.mi_cache_evict(view, other, keep, recent, span, ws.data_ptr(), ws.numel(),
                                         _lib.raw_stream(device.index)), "mi_cache_evict")
-        self._set_bound(target, min(keep, self.sizes[name] if name in self._captured else self._bound(name)))
+        if name in self._captured:
+            bound = self.sizes[name]
+        self._set_bound(target, min(keep, bound))
+        # rows moved, for all the host knows, unless there are no more than `keep`: then they are as they were
+        moved, self._pushed[target] = bound > keep, 0 if bound > keep else self._told(name)
+        if moved or name not in self._loaded:
+            self._loaded.discard(target)
+        else:
+            self._loaded.add(target)
+        if captured and (moved or name in self._mixed):
+            self._mixed.add(target)
 
     def trim(self, name, lengths=0):
         """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
@@ -315,11 +374,13 @@ class CacheBank(nn.Module):
                 raise ValueError(f"CacheBank.trim: lengths must not be negative, got {number}")
             number = min(number, self.sizes[name])
         with _on(device):
-            self._changes(name)
+            captured = self._changes(name)
             _lib.check(_lib.lib().mi_cache_trim(view, None if each is None else each.data_ptr(), number,
                                                 _lib.raw_stream(device.index)), "mi_cache_trim")
         bound = self._bound(name)
         self._set_bound(name, bound if each is not None else min(number, bound))
+        if self._pushed[name] is not None:             # an empty bank is in order
+            self._pushed[name] = None if each is None and number == 0 and not captured else 0
 
     def __getitem__(self, name):
         """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""

@@ -266,6 +266,21 @@ __global__ __launch_bounds__(256) void cache_longest_kernel(PushParams p, int *o
     if (threadIdx.x == 0) *out = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
 }
 
+// Clears *out where the last rows of a (sequence, head) are not the rows pushed last, in their order: what causal attention of several
+// rows goes by.  A sequence of which no row was evicted is in order.
+__global__ void cache_order_start_kernel(int *out) { *out = 1; }
+
+__global__ __launch_bounds__(256) void cache_order_kernel(PushParams p, int *out)
+{
+    const long long bh = blockIdx.x;
+    const int b = (int)(bh / p.c.heads), len = rows_used(p.c, b), seen = p.c.seen[b];
+    int n = p.counts ? p.counts[b] : p.T;
+    n = n > p.T ? p.T : n;
+    if (n <= 1 || seen == len) return;
+    for (int slot = max(0, len - n) + (int)threadIdx.x; slot < len; slot += 256)
+        if (p.c.position[bh * p.c.rows + slot] != seen - len + slot) *out = 0;
+}
+
 // Every sequence is cut to at most its entry of `lengths` (or `length`): of each head the rows pushed last leave.  Where no row of the
 // sequence was ever evicted, or what leaves lies behind the new length in the order of its pushes, that is all there is to do.  An
 // eviction puts rows from above into freed slots, so that a row's slot says nothing of its age: then the rows with the largest positions

@@ -268,6 +268,21 @@ int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, 
     return MI_OK;
 }
 
+int mi_cache_in_order(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream)
+{
+    MI_TRY(check_cache(cache, "mi_cache_in_order"));
+    if (!out) return fail(MI_ERR_ARG, "mi_cache_in_order: null pointer");
+    if (T < 0 || T > MAX_ROWS) return fail(MI_ERR_ARG, "mi_cache_in_order: bad T=%lld", (long long)T);
+    mi::PushParams p{};
+    p.c = view(cache);
+    p.counts = counts;
+    p.T = (int)T;
+    hipLaunchKernelGGL(mi::cache_order_start_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, out);
+    hipLaunchKernelGGL(mi::cache_order_kernel, dim3((unsigned)(cache->batch * cache->heads)), dim3(256), 0, (hipStream_t)stream, p, out);
+    HIP_CHECK(hipGetLastError());
+    return MI_OK;
+}
+
 int mi_cache_trim(const mi_cache_t *cache, const int32_t *lengths, int64_t length, mi_stream_t stream)
 {
     MI_TRY(check_cache(cache, "mi_cache_trim"));

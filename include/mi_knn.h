@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MI_ABI_VERSION 9
+#define MI_ABI_VERSION 10
 
 enum { MI_OK = 0, MI_ERR_ARG = -1, MI_ERR_HIP = -2, MI_ERR_WORKSPACE = -3, MI_ERR_UNSUPPORTED = -4 };
 enum { MI_F32 = 0, MI_BF16 = 1 };            /* compute dtype of the similarity GEMM            */
@@ -258,6 +258,10 @@ int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_s
 /* *out (device) = the most rows that a sequence would have after mi_cache_push of these counts, whether they fit or not. */
 int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream);
 
+/* *out (device) = 1 if the last rows of every sequence and head, T of them or counts[b], are the rows pushed last, in their order, else
+ * 0: what causal mi_cache_attend of several rows goes by.  It is so until rows are evicted, and then of the rows pushed since. */
+int mi_cache_in_order(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream);
+
 /* length[b] = min(length[b], lengths[b]) (device int32[batch]; NULL: `length` for all): of each head the rows pushed last leave, by
  * position.  Where an eviction has left them in slots below the new length, these take, in ascending order, the rows that stay of the
  * slots above.  Positions go on from the cut, and behind every row that stays (a head that evicted some of the rows pushed last loses
@@ -270,7 +274,8 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
 /* Softmax attention of T query rows of heads * group query heads over the bank; query head h reads head h / group.
  *   out[b, h, t] = sum_s p[s] value[s],  p = softmax over the visible slots s of scale * query[b, h, t] . key[s]
  * Row t of sequence b is real if t < counts[b] (NULL: all T).  causal: the last counts[b] rows of the sequence are the query rows
- * themselves, so row t sees the slots before length[b] - counts[b] + t + 1; otherwise all of length[b].  A row that is not real
+ * themselves, in order (mi_cache_in_order: several rows attend after their push and before the next eviction), so row t sees the
+ * slots before length[b] - counts[b] + t + 1; otherwise all of length[b].  A row that is not real
  * or sees nothing gives zeros.  accumulate: weight[b, h, s] += the sum of p[s] over the real rows and the group's heads.
  * query, out: [batch][heads * group][T][dim] of `dtype` with strides as in mi_cache_push.  Products are exact in bf16 pieces of
  * the query (one for bf16, two for float16, three for float32), sums and softmax statistics are float32.

@@ -238,3 +238,195 @@ def test_push_does_not_look_where_lengths_are_known():
         assert len(looks) == 1 and bank.lengths("kv").tolist() == [51, 51]
     finally:
         L.mi_cache_longest = real
+
+
+# ------------------------------------------------------------------------------------------------------ attend after an eviction
+def _query(rs, ref, T, group=2):
+    return _rand(rs, (ref.batch, ref.heads * group, T, ref.dim), "bf16", 0.3)
+
+
+@gpu
+def test_causal_attention_refuses_rows_that_an_eviction_moved():
+    """Push a draft, evict, attend: the draft's rows are not the last ones any more, so that slots say nothing of who sees whom."""
+    rs = np.random.RandomState(3)
+    bank, ref = _aged(rs, 1, 2, 64, 20, 12)
+    _push(bank, ref, rs, 4)
+    bank.weights("kv")[..., :16] = torch.arange(16.0)
+    for h in range(2):
+        ref.weight[0][h] = np.arange(16.0)
+    bank.evict("kv", 12, recent=4)
+    ref.evict(12, 4)
+    _rows_equal(bank, ref)
+    assert list(ref.position[0][0]) == [12, 13, 14, 15, *range(4, 12)]
+    q = _query(rs, ref, 4)
+    before = bank.weights("kv").clone()
+    for call in (dict(), dict(accumulate=True), dict(counts=[3]), dict(counts=torch.tensor([4], device="cuda"))):
+        with pytest.raises(RuntimeError, match="evict"):
+            bank.attend("kv", q.cuda(), **call)
+    assert torch.equal(bank.weights("kv"), before)
+    on_device = q.cuda()
+    with pytest.raises(RuntimeError, match="evict"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+        bank.attend("kv", on_device)
+    # what does not go by the order of the rows: one row, rows that all see everything, no order at all
+    _check_out(bank.attend("kv", q[:, :, :1].cuda()), *ref.attend(_np(q[:, :, :1])), "bf16")
+    _check_out(bank.attend("kv", q.cuda(), counts=[1]), *ref.attend(_np(q), [1]), "bf16")
+    _check_out(bank.attend("kv", q.cuda(), causal=False), *ref.attend(_np(q), causal=False), "bf16")
+    # rows pushed since are in order, and a copy of the bank, or its state in another one, is as mixed as the bank
+    twin = _bank(1, 2, 64, 20)
+    twin.load_state_dict(bank.state_dict())
+    for other in (twin, copy.deepcopy(bank)):
+        with pytest.raises(RuntimeError, match="evict"):
+            other.attend("kv", q.cuda())
+    _push(bank, ref, rs, 4)
+    _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
+    bank.trim("kv", 13)
+    ref.trim(13)
+    with pytest.raises(RuntimeError, match="evict"):
+        bank.attend("kv", q.cuda())
+    bank.trim("kv")
+    ref.trim(0)
+    _push(bank, ref, rs, 6)
+    _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
+
+
+@gpu
+def test_causal_attention_after_an_eviction_that_left_the_last_rows_in_order():
+    """The device says whether the last rows are in their order: an eviction that moved nothing, or older rows only, stands in no one's way."""
+    rs = np.random.RandomState(4)
+    bank, ref = _aged(rs, 2, 1, 64, 40, 30)
+    q = _query(rs, ref, 3)
+    bank.trim("kv", torch.tensor([20, 20], device="cuda"))                               # the host still counts 30 rows
+    ref.trim([20, 20])
+    bank.evict("kv", 20)
+    _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
+    for b, n in enumerate((20, ref.length(1))):                                          # one old row leaves, the youngest takes its slot: one is enough
+        ref.weight[b][0] = np.arange(n) + 1.0
+        bank.weights("kv")[b, 0, :n] = torch.arange(n) + 1.0
+    keep = 19
+    bank.evict("kv", keep)
+    ref.evict(keep)
+    assert list(ref.position[0][0]) == [19, *range(1, 19)]
+    with pytest.raises(RuntimeError, match="evict"):
+        bank.attend("kv", q.cuda())
+    bank.register("small", dim=64, k=20, batch=2)
+    bank.evict("kv", keep, into="small")                                                 # as it is, the mixed order with it
+    with pytest.raises(RuntimeError, match="evict"):
+        bank.attend("small", q.cuda())
+    _push(bank, ref, rs, 5, [5, 3])
+    _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
+    _check_out(bank.attend("kv", q.cuda(), counts=[2, 3]), *ref.attend(_np(q), [2, 3]), "bf16")
+
+
+@gpu
+def test_the_look_at_the_order_is_needed_once():
+    """A restored state is looked at before its first causal attention over several rows; pushes and attention go on without."""
+    rs = np.random.RandomState(5)
+    bank, ref = _aged(rs, 1, 1, 64, 64, 40)
+    other = _bank(1, 1, 64, 64)
+    other.load_state_dict(bank.state_dict())
+    looks, look = [], other._in_order
+
+    def counting(*args):
+        looks.append(1)
+        return look(*args)
+    other._in_order = counting
+    q = _query(rs, ref, 8)
+    for counts in (None, [3], None):
+        _check_out(other.attend("kv", q.cuda(), counts=counts), *ref.attend(_np(q), counts), "bf16")
+    assert len(looks) == 1
+    other.evict("kv", 30)
+    kv = torch.zeros(1, 1, 8, 64, device="cuda")
+    for _ in range(2):
+        other.push("kv", kv, kv)
+        other.attend("kv", q.cuda())
+    assert len(looks) == 1
+
+
+@gpu
+def test_order_of_rows_and_graphs():
+    """A graph's pushes stand before its own attention; what a replay may have evicted is looked at outside of it."""
+    rs = np.random.RandomState(9)
+    bank, ref = _aged(rs, 1, 1, 64, 64, 40)
+    kv = [torch.zeros(1, 1, 3, 64, device="cuda") for _ in range(2)]
+    q = _query(rs, ref, 3)
+    on_device = q.cuda()
+
+    def step():
+        bank.push("kv", *kv)
+        out = bank.attend("kv", on_device)
+        bank.evict("kv", 30)
+        return out
+    step()
+    graphs = []
+    for _ in range(2):                                                                   # captured twice: an eviction stands before the second
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    ref.push(_np(kv[0]), _np(kv[1]))
+    ref.evict(30)
+    for i in range(4):
+        rows = [torch.from_numpy(rs.randn(1, 1, 3, 64).astype(np.float32)) for _ in range(2)]
+        for t, x in zip(kv, rows):
+            t.copy_(x)
+        bank.weights("kv").copy_(torch.rand(64, generator=torch.Generator().manual_seed(i)))
+        ref.weight[0][0] = _np(bank.weights("kv"))[0, 0, :30]
+        ref.push(_np(rows[0]), _np(rows[1]))
+        want = ref.attend(_np(q))
+        g, out = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        _check_out(out, *want, "bf16")
+        ref.evict(30)
+        _rows_equal(bank, ref)
+        if list(ref.position[0][0][-3:]) != list(range(ref.seen[0] - 3, ref.seen[0])):
+            with pytest.raises(RuntimeError, match="evict"):
+                bank.attend("kv", on_device)
+    _push(bank, ref, rs, 4)
+    _check_out(bank.attend("kv", on_device), *ref.attend(_np(q)), "bf16")
+    state = bank.state_dict()
+    twin = _bank(1, 1, 64, 64)
+    twin.load_state_dict(state)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):                                                            # a loaded state is taken to be in order: a graph cannot look
+        out = twin.attend("kv", on_device)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        _check_out(out, *ref.attend(_np(q)), "bf16")
+
+
+@gpu
+def test_order_of_rows_through_the_c_abi():
+    import ctypes
+    ica = _ica()
+    L = ica._lib.lib()
+    rs = np.random.RandomState(6)
+    bank, _ = _aged(rs, 3, 2, 64, 64, 50)
+    bank.trim("kv", torch.tensor([50, 9, 0], device="cuda"))
+    view, held = bank._cache("kv", "test")
+    out = torch.full((1,), 7, dtype=torch.int32, device="cuda")
+
+    def ask(T, counts=None):
+        c = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+        assert L.mi_cache_in_order(view, None if c is None else c.data_ptr(), T, out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        return int(out)
+    assert ask(1) == ask(5) == ask(64) == 1
+    held[7][0] += 10                                                                     # rows left the first sequence
+    held[5][0, :, :50] += 10
+    assert ask(50) == 1
+    held[5][0, 1, 45] = 3
+    assert ask(4) == 1 and ask(5) == 0 and ask(64) == 0 and ask(8, [4, 8, 8]) == 1 and ask(8, [8, 0, 0]) == 0 and ask(8, [-1, 9, 1]) == 1
+    held[5][0, 1, 45] = 55
+    held[5][0, 1, 49] = 0
+    assert ask(1) == 1 and ask(2) == 0                                                   # one row sees everything, whatever the order
+
+
+def test_abi_refuses_a_bad_look_at_the_order():
+    import ctypes
+    ica = _ica()
+    L, at = ica._lib.lib(), 1 << 20
+    cache = ctypes.byref(ica._lib.Cache(at, at, at, at, at, at, at, at, 2, 2, 64, 64, 60))
+    assert L.mi_cache_in_order(cache, None, 1, None, None) == -1 and L.mi_cache_in_order(cache, None, -1, at, None) == -1
+    assert L.mi_cache_in_order(None, None, 1, at, None) == -1 and b"null cache" in L.mi_last_error()
