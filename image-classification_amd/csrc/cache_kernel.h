@@ -256,8 +256,9 @@ __global__ __launch_bounds__(256) void cache_longest_kernel(PushParams p, int *o
     __shared__ int s_most[4];
     int most = 0;
     for (int b = threadIdx.x; b < p.c.batch; b += 256) {
-        const int n = p.counts ? p.counts[b] : p.T;
-        most = max(most, rows_used(p.c, b) + (n < 0 ? 0 : n > p.T ? p.T : n));
+        int n = p.counts ? p.counts[b] : p.T;
+        n = n < 0 ? 0 : n > p.T ? p.T : n;
+        most = max(most, (int)min((uint32_t)rows_used(p.c, b) + (uint32_t)n, 0x7fffffffu));     // up to 2^30 each
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));

@@ -255,7 +255,8 @@ int64_t mi_cache_width(int64_t dim);
 int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_strides, const void *value, const int64_t *value_strides,
                   int dtype, int64_t T, const int32_t *counts, void *held_key, void *held_value, mi_stream_t stream);
 
-/* *out (device) = the most rows that a sequence would have after mi_cache_push of these counts, whether they fit or not. */
+/* *out (device) = the most rows that a sequence would have after mi_cache_push of these counts, whether they fit or not
+ * (at most 2^31 - 1). */
 int mi_cache_longest(const mi_cache_t *cache, const int32_t *counts, int64_t T, int32_t *out, mi_stream_t stream);
 
 /* *out (device) = 1 if the last rows of every sequence and head, T of them or counts[b], are the rows pushed last, in their order, else

@@ -430,3 +430,19 @@ def test_abi_refuses_a_bad_look_at_the_order():
     cache = ctypes.byref(ica._lib.Cache(at, at, at, at, at, at, at, at, 2, 2, 64, 64, 60))
     assert L.mi_cache_in_order(cache, None, 1, None, None) == -1 and L.mi_cache_in_order(cache, None, -1, at, None) == -1
     assert L.mi_cache_in_order(None, None, 1, at, None) == -1 and b"null cache" in L.mi_last_error()
+
+
+@gpu
+def test_longest_does_not_run_over():
+    """The most rows a bank may hold and the most a push may bring: their sum is 2^31, which an int cannot say."""
+    import ctypes
+    ica = _ica()
+    L = ica._lib.lib()
+    length = torch.tensor([1 << 30, 5], dtype=torch.int32, device="cuda")
+    out = torch.zeros(1, dtype=torch.int32, device="cuda")
+    at = out.data_ptr()                                                                  # (only lengths and counts are read)
+    base = -(-at // 16) * 16
+    view = ica._lib.Cache(base, base, base, base, base, base, length.data_ptr(), base, 2, 1, 64, 1 << 30, 1 << 30)
+    for T, want in ((1 << 30, 2 ** 31 - 1), ((1 << 30) - 1, 2 ** 31 - 1), (7, (1 << 30) + 7)):
+        assert L.mi_cache_longest(ctypes.byref(view), None, T, out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        assert int(out) == want
