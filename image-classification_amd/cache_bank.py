@@ -242,8 +242,8 @@ class CacheBank(nn.Module):
 
         ``counts`` (one whole number for each sequence, a list or a tensor on the device): only the first ``counts[b]`` of the T rows
         of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now holds for the two, in
-        their type and [batch, heads, T, dim], zeros where nothing was stored.  Raises ``RuntimeError`` before anything is written if a
-        sequence would pass ``k`` rows."""
+        their type and [batch, heads, T, dim], zeros where nothing was stored (float16 above 57344 is held as 65536, and returned as 65504).
+        Raises ``RuntimeError`` before anything is written if a sequence would pass ``k`` rows."""
         view, held_by = self._cache(name, "push")
         device = held_by[0].device
         heads = self.shapes[name][1]

@@ -225,7 +225,9 @@ __global__ __launch_bounds__(256) void cache_push_kernel(PushParams p)
             for (int i = 0; i < 8; ++i) {
                 const int four = (int)(code >> (4 * i)) & 15, low = four & 7;
                 const float a = (low < 4 ? 0.5f * (float)low : low < 6 ? (float)(low - 2) : (float)(2 * low - 8)) * s;
-                v[i] = poison ? __uint_as_float(0x7fc00000u) : !real ? 0.f : four > 7 ? -a : a;
+                // a float16 above 57344 is held as 2^16, past its largest number: the copy is the nearest that there is
+                const float near = DT == CACHE_F16 ? fminf(a, 65504.f) : a;
+                v[i] = poison ? __uint_as_float(0x7fc00000u) : !real ? 0.f : four > 7 ? -near : near;
             }
             const long long at_row = ((long long)b * p.c.heads + h) * p.T + t;
             store8<DT>(held + (at_row * p.c.dim + c * 8) * elem_bytes<DT>(), v);

@@ -251,7 +251,7 @@ int64_t mi_cache_width(int64_t dim);
  * taken as 0 .. T).  key, value: [batch][heads][T][dim] of `dtype`, strides in ELEMENTS for sequence, head and row (multiples of
  * 8 elements and 16-byte aligned rows); dims are contiguous.  Rows beyond `limit` are dropped.  The weight of a new row is 0.
  * held_key, held_value (contiguous [batch][heads][T][dim] of `dtype`, both or neither): the values that the bank now holds;
- * zeros for rows that were not stored. */
+ * zeros for rows that were not stored.  (A float16 above 57344 is held as 65536, and copied as 65504.) */
 int mi_cache_push(const mi_cache_t *cache, const void *key, const int64_t *key_strides, const void *value, const int64_t *value_strides,
                   int dtype, int64_t T, const int32_t *counts, void *held_key, void *held_value, mi_stream_t stream);
 

@@ -446,3 +446,23 @@ def test_longest_does_not_run_over():
     for T, want in ((1 << 30, 2 ** 31 - 1), ((1 << 30) - 1, 2 ** 31 - 1), (7, (1 << 30) + 7)):
         assert L.mi_cache_longest(ctypes.byref(view), None, T, out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
         assert int(out) == want
+
+
+
+# ------------------------------------------------------------------------------------------------------------ ends of the types
+@gpu
+def test_held_float16_rows_stay_finite():
+    """Above 7 * 2^13 the nearest value that 4 bits hold is 2^16, past the largest float16: what is returned saturates, what is held does not."""
+    f16 = np.float16
+    tops = [f16(57344), np.nextafter(f16(57344), f16(60000)), f16(60000), f16(65504), f16(-65504), f16(49152)]
+    x = np.zeros((1, 1, len(tops), 64), f16)
+    x[0, 0, :, 5] = tops
+    x[0, 0, :, 6] = f16(1000)
+    x[0, 0, :, 40] = f16(3)
+    bank, ref = _bank(1, 1, 64, 16), cr.RefBank(1, 1, 64, 16)
+    held = bank.push("kv", torch.from_numpy(x).cuda(), torch.from_numpy(-x).cuda(), held=True)
+    want = ref.push(x.astype(np.float64), -x.astype(np.float64))
+    assert np.abs(want[0]).max() == 65536
+    _rows_equal(bank, ref)
+    for got, w in zip(held, want):
+        _same(_np(got), np.clip(w, -65504, 65504))
