@@ -865,11 +865,13 @@ __global__ __launch_bounds__(256, 2) void cache_attend_kernel(CacheAttendParams 
                 store8<CACHE_F32>(p.part + g * W + d, x);
                 if (d == 0) p.part_ml[g] = make_float2(den == 0.f ? -INFINITY : rref, den);
             } else {
-                const float inv = 1.f / den;                      // (a row that sees nothing but NaN is NaN, one that sees nothing is zero)
-                for (int i = 0; i < 8; ++i) x[i] = den == 0.f ? 0.f : x[i] * inv;
+                // a row that sees nothing is zero; one that sees nothing but NaN, or whose scores are all -inf (0 / 0), is NaN
                 const int t = row / p.G, g = row - t * p.G;
+                const bool none = visible(t, n, len, p.causal) <= 0;
+                const float inv = 1.f / den;
+                for (int i = 0; i < 8; ++i) x[i] = none ? 0.f : x[i] * inv;
                 if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-                if (p.norm && d == 0) p.norm[bh * p.R + row] = make_float2(rref, den == 0.f ? 0.f : inv);
+                if (p.norm && d == 0) p.norm[bh * p.R + row] = make_float2(rref, none ? 0.f : inv);
             }
         }
     }
@@ -986,6 +988,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
     const int row = tile * ROWS + wave * 32 + c;
     const bool real = row < p.R && row / p.G < n;
     const int lim = real ? visible(row / p.G, n, len, p.causal) : 0x7fffffff;      // rows that are not real need no mask: nothing is kept of them
+    const unsigned long long seeing = __ballot(real && lim > 0);  // rows that see anything: for the end, in two scalar registers
     // the workgroup's first row sees least of its real ones, the last one most
     const int t_first = tile * ROWS / p.G, t_last = min(min(tile * ROWS + ROWS - 1, p.R - 1) / p.G, n - 1);
     const int least = t_last < t_first ? 0 : visible(t_first, n, len, p.causal), most = t_last < t_first ? 0 : visible(t_last, n, len, p.causal);
@@ -1124,7 +1127,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
     float sum = total.value();
     sum += __shfl_xor(sum, 32);
     if (row >= p.R) return;
-    const bool none = !real || sum == 0.f;                        // (a row that sees nothing but NaN is NaN)
+    const bool none = !(seeing >> lane & 1);                      // (a row that sees nothing but NaN, or scores of -inf, is NaN)
     const int tq = row / p.G, g = row - tq * p.G;
     if (p.nsplit > 1) {
         const long long gr = ((long long)split * bhs + bh) * p.R + row;
@@ -1136,7 +1139,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : NB == 8 || DT == CACHE
             for (int i = 0; i < NB; ++i) x[i] = o[i][r];
             store_n<CACHE_F32, NB>(to + (8 * (r >> 2) + 4 * l + (r & 3)) * NB, x);
         }
-        if (l == 0) p.part_ml[gr] = make_float2(none ? -INFINITY : ref == -INFINITY ? 0.f : ref, sum);
+        if (l == 0) p.part_ml[gr] = make_float2(none || sum == 0.f ? -INFINITY : ref == -INFINITY ? 0.f : ref, sum);
         return;
     }
     const float inv = 1.f / sum;
@@ -1161,13 +1164,17 @@ constexpr int CACHE_MAX_SPLIT = 256, CACHE_FEW_SPLITS = 8;
 template <int DT, int W>
 __device__ __forceinline__ void store_joined(const CacheAttendParams &p, long long g0, int d, float (&x)[8], float big, float den)
 {
-    const float inv = 1.f / den;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = big == -INFINITY ? 0.f : x[i] * inv;
     const long long bh = g0 / p.R;
     const int row = (int)(g0 % p.R), b = (int)(bh / p.c.heads), h = (int)(bh % p.c.heads), t = row / p.G, g = row - t * p.G;
+    float inv = 1.f / den, off = big;
+    if (big == -INFINITY) {                  // no piece has sums: the row sees nothing (zero), or all of its scores are -inf (0 / 0)
+        const bool none = visible(t, real_rows(p.counts, b, p.T), rows_used(p.c, b), p.causal) <= 0;
+        inv = none ? 0.f : __uint_as_float(0x7fc00000u), off = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= inv;
     if (d < p.c.dim) store8<DT>(p.out + b * p.out_s[0] + (long long)(h * p.G + g) * p.out_s[1] + t * p.out_s[2] + (long long)d * elem_bytes<DT>(), x);
-    if (p.norm && d == 0) p.norm[g0] = big == -INFINITY ? make_float2(0.f, 0.f) : make_float2(big, inv);
+    if (p.norm && d == 0) p.norm[g0] = make_float2(off, inv);
 }
 
 template <int DT, int W>

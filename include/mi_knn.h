@@ -277,7 +277,8 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
  * Row t of sequence b is real if t < counts[b] (NULL: all T).  causal: the last counts[b] rows of the sequence are the query rows
  * themselves, in order (mi_cache_in_order: several rows attend after their push and before the next eviction), so row t sees the
  * slots before length[b] - counts[b] + t + 1; otherwise all of length[b].  A row that is not real
- * or sees nothing gives zeros.  accumulate: weight[b, h, s] += the sum of p[s] over the real rows and the group's heads.
+ * or sees nothing gives zeros; one that sees a NaN, or whose scores are all -inf, gives NaN (as the softmax does, and in the sums).
+ * accumulate: weight[b, h, s] += the sum of p[s] over the real rows and the group's heads.
  * query, out: [batch][heads * group][T][dim] of `dtype` with strides as in mi_cache_push.  Products are exact in bf16 pieces of
  * the query (one for bf16, two for float16, three for float32), sums and softmax statistics are float32.
  * `span`: about how many rows are in use (it sizes the launch; the result is right for any span >= 1). */

@@ -466,3 +466,35 @@ def test_held_float16_rows_stay_finite():
     _rows_equal(bank, ref)
     for got, w in zip(held, want):
         _same(_np(got), np.clip(w, -65504, 65504))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim,T,group,fill,k", [(64, 1, 1, 40, 64), (72, 1, 2, 3000, 3000), (64, 40, 1, 60, 64), (128, 100, 2, 3000, 3000), (256, 3, 2, 700, 700), (72, 9, 2, 200, 200)])
+def test_scores_that_are_all_minus_infinity(dtype, dim, T, group, fill, k):
+    """A row that sees something and whose scores are all -inf has no softmax: NaN, as exp(-inf - -inf) says, and NaN for the sums that it
+    takes part in.  Scores of which only some are -inf are ordinary; a row that sees nothing is zeros all the same."""
+    rs = np.random.RandomState(dim + T)
+    kv = [_rand(rs, (1, 1, fill, dim), "bf16", 0.3) for _ in range(2)]
+    kv[0][0, 0, :, 3] = 1.0                                                              # every key has a positive entry there ...
+    kv[0][0, 0, :, :32] = kv[0][0, 0, :, :32].clamp(-2, 2)
+    q = _rand(rs, (1, group, T, dim), dtype, 0.3)
+    q[0, :, T // 2, 3] = -float("inf")                                                   # ... so that -inf makes -inf of all scores
+    for causal in (True, False):
+        for n in (None, [T // 2 + 1]):
+            bank, ref = _bank(1, 1, dim, k), cr.RefBank(1, 1, dim, k)
+            bank.push("kv", kv[0].cuda(), kv[1].cuda())
+            ref.push(_np(kv[0]), _np(kv[1]))
+            assert (ref.key[0][0][:, 3] > 0).all()
+            out = bank.attend("kv", q.cuda(), counts=n, causal=causal, accumulate=True)
+            real = T if n is None else n[0]
+            clean = q.clone()
+            clean[0, :, T // 2, 3] = 0.0
+            want, bound, weigh = ref.attend(_np(clean), n, causal=causal, accumulate=True)
+            want[:, :, T // 2] = np.nan
+            _check_out(out, want, bound, dtype, T * group)
+            w = _np(bank.weights("kv"))[0, 0, :fill]
+            sees = fill - real + T // 2 + 1 if causal else fill
+            assert np.isnan(w[:sees]).all() and not np.isnan(w[sees:]).any()
+            d = np.abs(w - ref.weight[0][0])[sees:]
+            assert (d <= weigh[0][0][sees:] + 1e-12).all()
