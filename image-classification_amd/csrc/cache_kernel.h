@@ -506,7 +506,8 @@ __device__ __forceinline__ int real_rows(const int *counts, int b, int T)
 }
 
 // 8 values as 1..3 bf16 pieces whose sum is the value: 8 bits of significand each (bf16: exact with one, float16: with two,
-// float32: with three).  A piece of an infinity or NaN is that value itself, the rest zero.
+// float32: with three; the first is at most the largest bf16, which the largest float32 would round past).  One piece of an infinity or
+// NaN is that value itself, those after it are zero.
 // Probabilities need no such care: what is left of a NaN is a NaN.
 template <int P, bool CARE = true>
 __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[P])
@@ -516,10 +517,12 @@ __device__ __forceinline__ void split_pieces(const float (&x)[8], cb16x8 (&out)[
         float v = x[i];
 #pragma unroll
         for (int k = 0; k < P; ++k) {
-            const __bf16 h = (__bf16)v;
+            constexpr float MOST = 0x1.fep127f;      // the largest bf16
+            const bool first = CARE && P == 3 && k == 0;          // (an infinity or NaN is left to the second piece)
+            const __bf16 h = (__bf16)(first ? __builtin_amdgcn_fmed3f(v, -MOST, MOST) : v);
             out[k][i] = h;
             v = v - (float)h;
-            if (CARE && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.f;
+            if (CARE && !first && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.f;
         }
     }
 }

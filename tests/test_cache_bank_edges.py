@@ -498,3 +498,26 @@ def test_scores_that_are_all_minus_infinity(dtype, dim, T, group, fill, k):
             assert np.isnan(w[:sees]).all() and not np.isnan(w[sees:]).any()
             d = np.abs(w - ref.weight[0][0])[sees:]
             assert (d <= weigh[0][0][sees:] + 1e-12).all()
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_float32_queries_up_to_the_largest(T):
+    """The largest float32 rounds to an infinity in bf16; its pieces must not."""
+    rs = np.random.RandomState(8)
+    top = np.finfo(np.float32).max
+    key = (rs.randn(1, 1, 50, 64) * 2.0 ** -120).astype(np.float32)
+    value = rs.randn(1, 1, 50, 64).astype(np.float32)
+    q = np.zeros((1, 1, T, 64), np.float32)
+    q[..., 0] = top
+    q[..., 1] = -top
+    q[..., 2] = np.float32(3.3961775e38)                                                 # the least that rounds up, and its neighbour below
+    q[..., 3] = np.nextafter(np.float32(3.3961775e38), np.float32(0))
+    bank, ref = _bank(1, 1, 64, 64), cr.RefBank(1, 1, 64, 64)
+    bank.push("kv", torch.from_numpy(key).cuda(), torch.from_numpy(value).cuda())
+    ref.push(key.astype(np.float64), value.astype(np.float64))
+    out = bank.attend("kv", torch.from_numpy(q).cuda(), scale=0.01, accumulate=True)
+    want, bound, weigh = ref.attend(q.astype(np.float64), scale=0.01, accumulate=True)
+    assert np.isfinite(want).all() and np.ptp(want[0, 0, -1]) > 0
+    _check_out(out, want, bound, "fp32", T)
+    assert (np.abs(_np(bank.weights("kv"))[0, 0, :50] - ref.weight[0][0]) <= weigh[0][0] + 1e-12).all()
