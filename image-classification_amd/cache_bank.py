@@ -27,6 +27,7 @@ import operator
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -294,7 +295,7 @@ class CacheBank(nn.Module):
         query = self._rows("attend", name, query, "query", None, device)
         if query.shape[1] == 0 or query.shape[1] % heads:
             raise ValueError(f"CacheBank.attend: {query.shape[1]} query heads are no multiple of the bank's {heads}")
-        if torch.is_grad_enabled() and query.requires_grad:
+        if (torch.is_grad_enabled() and query.requires_grad) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(query).tangent is not None):
             raise RuntimeError("CacheBank.attend has no gradient: call it under torch.no_grad() or with query.detach()")
         scale = dim ** -0.5 if scale is None else float(scale)
         query = query.detach()

@@ -521,3 +521,19 @@ def test_float32_queries_up_to_the_largest(T):
     assert np.isfinite(want).all() and np.ptp(want[0, 0, -1]) > 0
     _check_out(out, want, bound, "fp32", T)
     assert (np.abs(_np(bank.weights("kv"))[0, 0, :50] - ref.weight[0][0]) <= weigh[0][0] + 1e-12).all()
+
+
+@gpu
+def test_attend_refuses_a_forward_mode_tangent():
+    import torch.autograd.forward_ad as fwd
+    rs = np.random.RandomState(7)
+    bank, _ = _filled(rs, 1, 1, 64, 16, 16)
+    q = torch.randn(1, 1, 2, 64, device="cuda")
+    want = bank.attend("kv", q)
+    with fwd.dual_level():
+        assert torch.equal(bank.attend("kv", q), want)                                   # no tangent, no objection
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        with pytest.raises(RuntimeError, match="no gradient"):
+            bank.attend("kv", dual)
+        assert torch.equal(bank.attend("kv", dual.detach()), want)
+        assert torch.equal(bank.attend("kv", fwd.unpack_dual(dual).primal), want)
