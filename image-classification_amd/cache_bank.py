@@ -14,7 +14,8 @@ Storage is registered buffers (``<name>_key``, ``_key_scale``, ``_value``, ``_va
 layouts and the number format in ``include/mi_knn.h``), so ``.to(device)`` and ``state_dict`` behave as for the other banks.  Each rank holds
 its own sequences: nothing is gathered.  No gradients: the bank is memory, as the MoCo queue is.  No CPU path.
 
-Lengths live on the device and no call waits for it, except a ``push`` that may run over: the host knows an upper bound of the lengths and
+Lengths live on the device and no call waits for it, except to copy ``counts`` that are given as a list, for the order of rows after an
+eviction (see ``attend``), and for a ``push`` that may run over: the host knows an upper bound of the lengths and
 reads them back when that bound plus the new rows passes ``k``, or when torch has written to the lengths, or put others in their place,
 since it knew it.  (A collective or a kernel of one's own that writes to them in place goes unnoticed: load them with ``load_state_dict``
 or ``copy_``.)  All calls can be captured into a graph; a captured ``push`` cannot look, and rows that do not fit when it is replayed are
@@ -241,8 +242,8 @@ class CacheBank(nn.Module):
     def push(self, name, key, value, counts=None, held=False):
         """Appends ``key`` and ``value`` [batch, heads, T, dim] behind the last row of every sequence, quantised to 4 bits.
 
-        ``counts`` (one whole number for each sequence, a list or a tensor on the device): only the first ``counts[b]`` of the T rows
-        of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now holds for the two, in
+        ``counts`` (one whole number for each sequence, a list, which the host waits to copy, or a tensor on the device): only the first
+        ``counts[b]`` of the T rows of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now holds for the two, in
         their type and [batch, heads, T, dim], zeros where nothing was stored (float16 above 57344 is held as 65536, and returned as 65504).
         Raises ``RuntimeError`` before anything is written if a sequence would pass ``k`` rows."""
         view, held_by = self._cache(name, "push")
@@ -288,7 +289,13 @@ class CacheBank(nn.Module):
         again, unless the last rows are still in their order (the host then waits for the device once, as it does for a state that was
         loaded).  ``counts``: as in :meth:`push`, real rows of each sequence (after an eviction, the counts of the push).  Rows that are
         not real or see nothing give zeros.  ``scale``: positive, ``dim ** -0.5`` if not given.  ``accumulate`` adds to :meth:`weights`
-        what each row of the bank got, summed over query rows and the group's heads; :meth:`evict` goes by that."""
+        what each row of the bank got, summed over query rows and the group's heads; :meth:`evict` goes by that.  What query rows that are
+        trimmed later (a rejected draft) have added to other rows stays: attend to a draft without, and to what was accepted of it with
+        ``accumulate``, where that matters.
+
+        Sums and statistics are float32; probabilities enter the second product as bf16 pieces: three for a float32 query (2^-24 of each
+        is left out), two for float16 and for up to 32 rows (T times the group) of bfloat16 (2^-17), one for more rows of bfloat16 (2^-8,
+        half a step of that type)."""
         view, held_by = self._cache(name, "attend")
         device = held_by[0].device
         batch, heads, dim = self.shapes[name]
@@ -362,7 +369,8 @@ class CacheBank(nn.Module):
     def trim(self, name, lengths=0):
         """Cuts every sequence to at most ``lengths`` rows (a number for all, or one for each sequence as a tensor on the device): 0 empties
         the bank, a smaller length takes back the rows pushed last (a rejected draft), by position, wherever an eviction has put them:
-        freed slots below the new length take, in ascending order, the rows that stay from above.  Positions go on from the cut."""
+        freed slots below the new length take, in ascending order, the rows that stay from above.  Positions go on from the cut; weights
+        stay as they are, with what the rows that leave had added to others as queries."""
         view, held_by = self._cache(name, "trim")
         device = held_by[0].device
         each, number = None, 0

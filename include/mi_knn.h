@@ -281,6 +281,8 @@ int mi_cache_read(const mi_cache_t *cache, void *key, void *value, mi_stream_t s
  * accumulate: weight[b, h, s] += the sum of p[s] over the real rows and the group's heads.
  * query, out: [batch][heads * group][T][dim] of `dtype` with strides as in mi_cache_push.  Products are exact in bf16 pieces of
  * the query (one for bf16, two for float16, three for float32), sums and softmax statistics are float32.
+ * Probabilities enter the second product as bf16 pieces too: three for float32 (2^-24 of each p is left out), two for float16 and for
+ * up to 32 rows (T * group) of bf16 (2^-17), one for more rows of bf16 (2^-8, half a step of the type).
  * `span`: about how many rows are in use (it sizes the launch; the result is right for any span >= 1). */
 size_t mi_cache_attend_workspace_bytes(const mi_cache_t *cache, int dtype, int64_t T, int64_t group, int64_t span, int causal, int accumulate);
 int mi_cache_attend(const mi_cache_t *cache, const void *query, const int64_t *query_strides, void *out, const int64_t *out_strides,
