@@ -122,8 +122,9 @@ class CacheBank(nn.Module):
         self._captured.discard(name)
         self._mixed.discard(name)
         self._loaded.discard(name)
-        self._pushed[name] = None
-        self._set_bound(name, 0)
+        self._pushed[name] = 0
+        self._bound(name)
+        self._bounds[name], self._pushed[name] = 0, None
         self._views.pop(name, None)
 
     # ------------------------------------------------------------------------------------------------------------ helpers
@@ -188,17 +189,17 @@ class CacheBank(nn.Module):
 
     def _bound(self, name) -> int:
         """The bound, where it still speaks of the lengths that the bank has; otherwise they may be anything up to ``k``."""
-        held, length = self._marks.get(name, (None, None)), self._buffers[f"{name}_length"]
-        if held[0] is not length or held[1] != _mark(length):
-            self._set_bound(name, self.sizes[name])
+        length, (known, mark) = self._buffers[f"{name}_length"], self._marks.get(name, (None, None))
+        now = _mark(length)
+        if known is not length or mark != now:
+            self._marks[name], self._bounds[name] = (length, now), self.sizes[name]
             if self._pushed[name] is None:
                 self._loaded.add(name)
             self._pushed[name] = 0
         return self._bounds[name]
 
     def _set_bound(self, name, bound):
-        length = self._buffers[f"{name}_length"]
-        self._marks[name] = length, _mark(length)
+        """A bound after a call, of the lengths that :meth:`_bound` was last asked for before it."""
         self._bounds[name] = self.sizes[name] if name in self._captured else min(bound, self.sizes[name])
 
     def _span(self, name) -> int:
@@ -349,7 +350,7 @@ class CacheBank(nn.Module):
             raise ValueError(f"CacheBank.evict: recent={recent} outside [0, keep={keep}]")
         L = _lib.lib()
         with _on(device):
-            captured, bound = self._changes(target), self._bound(name)
+            captured, bound, _ = self._changes(target), self._bound(name), self._bound(target)
             ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(view, keep)), dtype=torch.uint8, device=device)
             span = self._span(name)
             _lib.check(L.mi_cache_evict(view, other, keep, recent, span, ws.data_ptr(), ws.numel(),
