@@ -71,12 +71,6 @@ def _aligned(t: torch.Tensor):
     return t, _strides(t)
 
 
-def _mark(t: torch.Tensor):
-    """Tells whether torch has written to ``t``, or it has come to lie elsewhere, since an earlier mark that this one equals.  Writes to an
-    inference tensor are not counted: no two of its marks are equal."""
-    return t.data_ptr(), object() if t.is_inference() else t._version
-
-
 def _part_shapes(k, batch, heads, dim):
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     rows = (k + 63) // 64 * 64
@@ -92,7 +86,7 @@ class CacheBank(nn.Module):
         self.sizes = {}            # name -> k
         self.shapes = {}           # name -> (batch, heads, dim)
         self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows ...
-        self._marks = {}           # name -> ... and the lengths that this was said of: (buffer, its mark)
+        self._marks = {}           # name -> ... and the lengths that this was said of: (buffer, torch's count of writes to it, where it starts)
         self._pushed = {}          # name -> rows pushed since slots may have stopped telling a row's age, or None: they tell it
         self._captured = set()     # names whose lengths a graph may change behind the host's back
         self._mixed = set()        # names whose rows a graph may put into another order
@@ -148,6 +142,8 @@ class CacheBank(nn.Module):
                                    f"got {t.dtype} on {t.device} (move banks with .to(device), not to another dtype)")
         starts = [t.data_ptr() for t in held]
         view = ctypes.pointer(_lib.Cache(*starts, batch, heads, dim, held[4].shape[2], self.sizes[name]))
+        if name in self._marks and self._marks[name][2] != starts[6]:
+            del self._marks[name]
         self._bound(name)
         self._views[name] = (held, view, pick, starts)
         return view, held
@@ -189,10 +185,11 @@ class CacheBank(nn.Module):
 
     def _bound(self, name) -> int:
         """The bound, where it still speaks of the lengths that the bank has; otherwise they may be anything up to ``k``."""
-        length, (known, mark) = self._buffers[f"{name}_length"], self._marks.get(name, (None, None))
-        now = _mark(length)
-        if known is not length or mark != now:
-            self._marks[name], self._bounds[name] = (length, now), self.sizes[name]
+        length, mark = self._buffers[f"{name}_length"], self._marks.get(name)
+        if mark is None or mark[0] is not length or mark[1] != length._version:
+            # (writes to an inference tensor are not counted: it has no mark that holds)
+            self._marks[name] = (None, 0, 0) if length.is_inference() else (length, length._version, length.data_ptr())
+            self._bounds[name] = self.sizes[name]
             if self._pushed[name] is None:
                 self._loaded.add(name)
             self._pushed[name] = 0
@@ -350,7 +347,9 @@ class CacheBank(nn.Module):
             raise ValueError(f"CacheBank.evict: recent={recent} outside [0, keep={keep}]")
         L = _lib.lib()
         with _on(device):
-            captured, bound, _ = self._changes(target), self._bound(name), self._bound(target)
+            captured, bound = self._changes(target), self._bound(name)
+            if into is not None:
+                self._bound(into)
             ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(view, keep)), dtype=torch.uint8, device=device)
             span = self._span(name)
             _lib.check(L.mi_cache_evict(view, other, keep, recent, span, ws.data_ptr(), ws.numel(),
