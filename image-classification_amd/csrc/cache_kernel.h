@@ -289,94 +289,100 @@ __global__ __launch_bounds__(256) void cache_order_kernel(PushParams p, int *out
 // eviction puts rows from above into freed slots, so that a row's slot says nothing of its age: then the rows with the largest positions
 // leave, and the slots that they free below the new length take the rows that stay from above it, both in ascending order (as an
 // eviction does; no row is read that another one is written to).  Positions go on from the cut, and in any case behind all that stay.
-// One workgroup a sequence: the order is looked at in 4 bytes a head and row that leaves; only a cut that finds rows out of order
-// goes over a bank, head by head.
-constexpr int TRIM_THREADS = 1024;
+// A workgroup a sequence, a wave a head: the order is looked at in 4 bytes a head and row that leaves (2.6 us for 64 sequences of 8 heads).
+// Only where it does not hold is a head gone over, without a barrier, in two passes where an eviction has kept all that leaves (a call that
+// takes 5 of 2048 rows back: 24 us for 64 sequences of 8 heads; of 131 k rows 530 us for one.  With a workgroup on one head after the
+// other and the edge found by digits, counted with atomics: 440 and 3800 us).
+constexpr int TRIM_THREADS = 1024, TRIM_RING = 512;
+constexpr int TRIM_NO_TIES = 0x7fffffff;
 
 struct TrimShared {
-    int hist[256], wave[TRIM_THREADS / 64];
-    int holes[2 * TRIM_THREADS], tails[TRIM_THREADS];
-    int pick[3], out_of_order, last;
+    int holes[TRIM_THREADS / 64][TRIM_RING], tails[TRIM_THREADS / 64][64];
+    int last;
 };
 
-// How many threads before this one have `mine` set, and how many have it in all.
-__device__ __forceinline__ int block_rank(bool mine, TrimShared &sh, int &all)
+// How many of the first `len` rows f says yes to (its argument: a row's position, in unsigned order).
+template <typename F>
+__device__ __forceinline__ int count_rows(const int *pos, int len, F f)
 {
-    const unsigned long long who = __ballot(mine);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
-    if (lane == 0) sh.wave[wave] = __popcll(who);
-    __syncthreads();
-    int before = __popcll(who & ((1ull << lane) - 1));
-    all = 0;
-    for (int i = 0; i < TRIM_THREADS / 64; ++i) {
-        if (i < wave) before += sh.wave[i];
-        all += sh.wave[i];
+    int n = 0;
+    for (int i0 = (threadIdx.x & 63) * 4; i0 < len; i0 += 1024) {
+        int4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = i0 + 256 * k < len ? *(const int4 *)(pos + i0 + 256 * k) : make_int4(0, 0, 0, 0);      // (rows are allocated in 64s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + 256 * k, y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n += i + e < len && f((uint32_t)y[e] ^ 0x80000000u);
+        }
     }
-    return before;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+    return n;
 }
 
-// Lets the `gone` youngest of the `len` rows of one head leave and puts the others into slots 0 .. n = len - gone.
-__device__ __forceinline__ void trim_head(const CacheView &c, long long bh, int width, int len, int n, TrimShared &sh)
+// One wave: lets the len - n youngest of the `len` rows of one head leave and puts the others into slots 0 .. n.  Returns the largest
+// position that stays, where it may be seen - (len - n) or more, else -1.
+__device__ __forceinline__ int trim_head(const CacheView &c, long long bh, int width, int len, int n, int seen, int *holes, int *tails)
 {
-    const int tid = threadIdx.x;
+    const int lane = threadIdx.x & 63, gone = len - n;
     int *const pos = c.position + bh * c.rows;
-    const auto age = [&](int slot) { return (uint32_t)pos[slot] ^ 0x80000000u; };      // in the order of the positions
-    // the position that the gone-th youngest row has, by digits of 8 bits from the top; `left` of the rows on it leave, the highest slots
-    uint32_t edge = 0;
-    int left = len - n, ties = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += TRIM_THREADS) sh.hist[i] = 0;
-        __syncthreads();
-        const uint32_t known = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-        for (int i = tid; i < len; i += TRIM_THREADS) {
-            const uint32_t u = age(i);
-            if ((u & known) == edge) atomicAdd(&sh.hist[u >> shift & 255u], 1);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int digit = 255, rest = left;
-            while (digit > 0 && sh.hist[digit] < rest) rest -= sh.hist[digit--];
-            sh.pick[0] = digit, sh.pick[1] = rest, sh.pick[2] = sh.hist[digit];
-        }
-        __syncthreads();
-        edge |= (uint32_t)sh.pick[0] << shift;
-        left = sh.pick[1];
-        ties = sh.pick[2];
-        __syncthreads();
+    bool moved = false;
+    for (int i = n + lane; i < len; i += 64) moved |= pos[i] != seen - len + i;
+    if (!__any(moved)) return -1;
+    // rows behind `edge` leave, and of those on it all but the `tied` lowest slots
+    uint32_t edge = ((uint32_t)(seen - gone) ^ 0x80000000u) - 1;
+    int tied = TRIM_NO_TIES, last = -1;
+    if (count_rows(pos, len, [&](uint32_t u) { return u > edge; }) != gone) {
+        // this head has evicted some of the rows pushed last: the gone-th largest position, by bits from the top
+        edge = 0;
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+            if (count_rows(pos, len, [&](uint32_t u) { return u >= (edge | bit); }) >= gone) edge |= bit;
+        const int behind = count_rows(pos, len, [&](uint32_t u) { return u > edge; });
+        tied = count_rows(pos, len, [&](uint32_t u) { return u == edge; }) - (gone - behind);
+        if (tied > 0) last = (int)(edge ^ 0x80000000u);
+        else
+            for (int i = lane; i < len; i += 64)
+                if (((uint32_t)pos[i] ^ 0x80000000u) < edge) last = max(last, pos[i]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) last = max(last, __shfl_xor(last, d));
     }
-    const int tied = ties - left;            // rows on the edge that stay: the lowest slots
-    // whether a row leaves, asked for TRIM_THREADS neighbours at a time in ascending order; `on` counts the rows on the edge so far
-    const auto leaves = [&](int slot, int end, int &on) {
-        const uint32_t u = slot < end ? age(slot) : 0u;
-        int all;
-        const int before = on + block_rank(slot < end && u == edge, sh, all);
-        on += all;
-        return slot < end && (u > edge || (u == edge && before >= tied));
+    const unsigned long long below = (1ull << lane) - 1;
+    const auto leaves = [&](bool in, uint32_t u, int &on) {        // of 64 neighbours, asked in ascending order; `on`: rows on the edge so far
+        if (tied == TRIM_NO_TIES) return in && u > edge;
+        const unsigned long long who = __ballot(in && u == edge);
+        const int before = on + __popcll(who & below);
+        on += __popcll(who);
+        return in && (u > edge || (u == edge && before >= tied));
     };
-    int on_hole = 0, on_tail = 0, all;
-    for (int i0 = 0; i0 < n; i0 += TRIM_THREADS) {
-        block_rank(i0 + tid < n && age(i0 + tid) == edge, sh, all);
-        on_tail += all;
-    }
+    int on_hole = 0, on_tail = tied == TRIM_NO_TIES ? 0 : count_rows(pos, n, [&](uint32_t u) { return u == edge; });
     const int words = width / 32, parts = 4 * words + 2;          // 16 bytes of key or value, or a byte of their scales, for each 32 dims
-    int found = 0, filled = 0, hole0 = 0;    // freed slots found, and taken; where the search goes on
-    for (int t0 = n; t0 < len; t0 += TRIM_THREADS) {
-        const bool stays = t0 + tid < len, gone = leaves(t0 + tid, len, on_tail);
-        const int at = block_rank(stays && !gone, sh, all);
-        const int tails = all;
-        if (stays && !gone) sh.tails[at] = t0 + tid;
-        while (found < filled + tails && hole0 < n) {             // as many freed slots as rows that stay: at most 2 TRIM_THREADS wait
-            const bool hole = leaves(hole0 + tid, n, on_hole);
-            const int k = block_rank(hole, sh, all);
-            if (hole) sh.holes[(found + k) % (2 * TRIM_THREADS)] = hole0 + tid;
-            found += all;
-            hole0 += TRIM_THREADS;
+    int found = 0, filled = 0, hole0 = 0;                          // freed slots found, and taken; where the search goes on
+    for (int t0 = n; t0 < len; t0 += 64) {
+        const bool in = t0 + lane < len, stays = in && !leaves(in, in ? (uint32_t)pos[t0 + lane] ^ 0x80000000u : 0u, on_tail);
+        const unsigned long long who = __ballot(stays);
+        if (!who) continue;
+        const int want = __popcll(who);
+        if (stays) tails[__popcll(who & below)] = t0 + lane;
+        while (found < filled + want && hole0 < n) {               // as many freed slots as rows that stay: fewer than 64 + 256 wait
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[k] = hole0 + 64 * k + lane < n ? (uint32_t)pos[hole0 + 64 * k + lane] ^ 0x80000000u : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int slot = hole0 + 64 * k + lane;
+                const bool hole = leaves(slot < n, u[k], on_hole);
+                const unsigned long long free = __ballot(hole);
+                if (hole) holes[(found + __popcll(free & below)) % TRIM_RING] = slot;
+                found += __popcll(free);
+            }
+            hole0 += 256;
         }
-        __syncthreads();
-        const int moves = min(tails, found - filled);
-        for (int i = tid; i < moves * parts; i += TRIM_THREADS) {
-            const int k = i / parts, part = i - k * parts, src = sh.tails[k], dst = sh.holes[(filled + k) % (2 * TRIM_THREADS)];
+        __threadfence_block();                                     // lists of the wave's own: written before they are read
+        const int moves = min(want, found - filled);
+        for (int i = lane; i < moves * parts; i += 64) {
+            const int k = i / parts, part = i - k * parts, src = tails[k], dst = holes[(filled + k) % TRIM_RING];
             if (part < 2 * words) {
                 uint8_t *side = (part < words ? c.key : c.value) + bh * c.rows * (width / 2) + part % words * 16;
                 *(uint4 *)(side + (long long)dst * (width / 2)) = *(const uint4 *)(side + (long long)src * (width / 2));
@@ -387,35 +393,28 @@ __device__ __forceinline__ void trim_head(const CacheView &c, long long bh, int 
             else pos[dst] = pos[src];
         }
         filled += moves;
-        __syncthreads();
+        __threadfence_block();                                     // and read before the next ones are written
     }
-    int last = -1;                           // of the rows that stay
-    for (int i = tid; i < n; i += TRIM_THREADS) last = max(last, pos[i]);
-    atomicMax(&sh.last, last);
+    return last;
 }
 
 __global__ __launch_bounds__(TRIM_THREADS) void cache_trim_kernel(CacheView c, const int *lengths, int length, int width)
 {
     __shared__ TrimShared sh;
-    const int b = blockIdx.x, tid = threadIdx.x;
+    const int b = blockIdx.x, wave = threadIdx.x >> 6;
     int n = lengths ? lengths[b] : length;
     n = n < 0 ? 0 : n;
     const int len = rows_used(c, b), gone = len - n, seen = c.seen[b];
     if (gone <= 0) return;
-    if (tid == 0) sh.out_of_order = 0, sh.last = -1;
+    if (threadIdx.x == 0) sh.last = -1;
     __syncthreads();
-    if (n > 0 && seen != len) {
-        const long long all = (long long)c.heads * gone;
-        for (long long i = tid; i < all; i += TRIM_THREADS) {
-            const int h = (int)(i / gone), slot = n + (int)(i - (long long)h * gone);
-            if (c.position[((long long)b * c.heads + h) * c.rows + slot] != seen - len + slot) sh.out_of_order = 1;
+    if (n > 0 && seen != len)
+        for (int h = wave; h < c.heads; h += TRIM_THREADS / 64) {
+            const int last = trim_head(c, (long long)b * c.heads + h, width, len, n, seen, sh.holes[wave], sh.tails[wave]);
+            if (last >= 0 && (threadIdx.x & 63) == 0) atomicMax(&sh.last, last);
         }
-        __syncthreads();
-        if (sh.out_of_order)
-            for (int h = 0; h < c.heads; ++h) trim_head(c, (long long)b * c.heads + h, width, len, n, sh);
-    }
     __syncthreads();
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
         c.length[b] = n;
         c.seen[b] = max(seen - gone, sh.last + 1);
     }
