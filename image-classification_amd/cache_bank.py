@@ -14,12 +14,11 @@ Storage is registered buffers (``<name>_key``, ``_key_scale``, ``_value``, ``_va
 layouts and the number format in ``include/mi_knn.h``), so ``.to(device)`` and ``state_dict`` behave as for the other banks.  Each rank holds
 its own sequences: nothing is gathered.  No gradients: the bank is memory, as the MoCo queue is.  No CPU path.
 
-Lengths live on the device and no call waits for it, except to copy ``counts`` that are given as a list, for the order of rows after an
-eviction (see ``attend``), and for a ``push`` that may run over: the host knows an upper bound of the lengths and
-reads them back when that bound plus the new rows passes ``k``, or when torch has written to the lengths, or put others in their place,
-since it knew it.  (A collective or a kernel of one's own that writes to them in place goes unnoticed: load them with ``load_state_dict``
-or ``copy_``.)  All calls can be captured into a graph; a captured ``push`` cannot look, and rows that do not fit when it is replayed are
-dropped."""
+Lengths live on the device and no call waits for it, except to copy ``counts`` that are given as a list, to look at the order of rows
+after an eviction (see ``attend``), and for a ``push`` that may run over: the host knows an upper bound of the lengths and reads them back
+when that bound plus the new rows passes ``k``, or when torch has written to the lengths, or put others in their place, since it knew it.
+(A collective or a kernel of one's own that writes to them in place goes unnoticed: load them with ``load_state_dict`` or ``copy_``.)  All
+calls can be captured into a graph; a captured ``push`` cannot look, and rows that do not fit when it is replayed are dropped."""
 from __future__ import annotations
 
 import contextlib
@@ -241,8 +240,9 @@ class CacheBank(nn.Module):
         """Appends ``key`` and ``value`` [batch, heads, T, dim] behind the last row of every sequence, quantised to 4 bits.
 
         ``counts`` (one whole number for each sequence, a list, which the host waits to copy, or a tensor on the device): only the first
-        ``counts[b]`` of the T rows of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now holds for the two, in
-        their type and [batch, heads, T, dim], zeros where nothing was stored (float16 above 57344 is held as 65536, and returned as 65504).
+        ``counts[b]`` of the T rows of sequence b are real; the others are not stored.  ``held=True`` returns the values that the bank now
+        holds for the two, in their type and [batch, heads, T, dim], zeros where nothing was stored (a float16 above 57344 is held as 65536,
+        and returned as 65504).
         Raises ``RuntimeError`` before anything is written if a sequence would pass ``k`` rows."""
         view, held_by = self._cache(name, "push")
         device = held_by[0].device
@@ -252,11 +252,15 @@ class CacheBank(nn.Module):
         if key.shape != value.shape or key.dtype != value.dtype:
             raise ValueError(f"CacheBank.push: key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} differ")
         T, k = key.shape[2], self.sizes[name]
+        least = T                                       # rows that every sequence gets, for all the host knows of a tensor
+        if counts is not None and not isinstance(counts, torch.Tensor):
+            counts = [int(n) for n in counts]
+            least = min(counts, default=T)
         counts = self._counts(counts, key.shape[0], T, device)
         with _on(device):
             if not self._changes(name):
                 bound = k if name in self._captured else self._bound(name)
-                if bound + T > k:                       # the one place that waits for the device
+                if bound + T > k:                       # waits for the device
                     longest = torch.empty(1, dtype=torch.int32, device=device)
                     _lib.check(_lib.lib().mi_cache_longest(view, None if counts is None else counts.data_ptr(), T, longest.data_ptr(),
                                                            _lib.raw_stream(device.index)), "mi_cache_longest")
@@ -274,7 +278,7 @@ class CacheBank(nn.Module):
                                                 None if counts is None else counts.data_ptr(), None if not held else out[0].data_ptr(),
                                                 None if not held else out[1].data_ptr(), _lib.raw_stream(device.index)), "mi_cache_push")
             if self._pushed[name] is not None:
-                self._pushed[name] += T
+                self._pushed[name] += least
         return out if held else None
 
     def attend(self, name, query, counts=None, scale=None, causal=True, accumulate=False):

@@ -537,3 +537,28 @@ def test_attend_refuses_a_forward_mode_tangent():
             bank.attend("kv", dual)
         assert torch.equal(bank.attend("kv", dual.detach()), want)
         assert torch.equal(bank.attend("kv", fwd.unpack_dual(dual).primal), want)
+
+
+@gpu
+def test_the_order_after_an_eviction_goes_by_the_fewest_rows_pushed():
+    """A list of counts says how many rows each sequence got: where one got fewer than the query has, its older rows are looked at."""
+    rs = np.random.RandomState(10)
+    bank, ref = _aged(rs, 2, 1, 64, 40, 30)
+    bank.trim("kv", 20)
+    ref.trim(20)
+    _push(bank, ref, rs, 8)
+    for b in range(2):
+        n = ref.length(b)
+        bank.weights("kv")[b, 0, :n] = torch.arange(n) + 1.0
+        ref.weight[b][0] = np.arange(n) + 1.0
+    keep = min(ref.length(b) for b in range(2)) - 2
+    bank.evict("kv", keep)
+    ref.evict(keep)
+    assert list(ref.position[1][0][-2:]) != [ref.seen[1] - 2, ref.seen[1] - 1]
+    _push(bank, ref, rs, 4, [4, 1])
+    q = _query(rs, ref, 4)
+    with pytest.raises(RuntimeError, match="evict"):
+        bank.attend("kv", q.cuda())
+    _check_out(bank.attend("kv", q.cuda(), counts=[4, 1]), *ref.attend(_np(q), [4, 1]), "bf16")
+    _push(bank, ref, rs, 4, np.array([4, 4]))
+    _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
