@@ -86,7 +86,8 @@ class CacheBank(nn.Module):
         self.shapes = {}           # name -> (batch, heads, dim)
         self._bounds = {}          # name -> rows that the longest sequence has at most, as far as the host knows ...
         self._marks = {}           # name -> ... and the lengths that this was said of: (buffer, torch's count of writes to it, where it starts)
-        self._pushed = {}          # name -> rows pushed since slots may have stopped telling a row's age, or None: they tell it
+        self._pushed = {}          # name -> rows pushed to every sequence since slots may have stopped telling a row's age, or None: they tell it
+        self._padded = {}          # name -> more rows of that time, of which counts on the device say how many there were
         self._captured = set()     # names whose lengths a graph may change behind the host's back
         self._mixed = set()        # names whose rows a graph may put into another order
         self._loaded = set()       # names whose rows came from elsewhere, in an order that the host has not seen
@@ -97,7 +98,9 @@ class CacheBank(nn.Module):
 
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
-        self._bounds, self._pushed, self._loaded = dict(self.sizes), dict.fromkeys(self.sizes, 0), set(self.sizes)
+        self._bounds, self._loaded = dict(self.sizes), set(self.sizes)
+        for name in self.sizes:
+            self._doubt(name)
 
     def register(self, name, dim, k, heads=1, batch=1, device=None):
         """An empty bank of ``k`` rows of ``dim`` values (a multiple of 8, at most 256) for each head of each sequence, on ``device``
@@ -115,7 +118,7 @@ class CacheBank(nn.Module):
         self._captured.discard(name)
         self._mixed.discard(name)
         self._loaded.discard(name)
-        self._pushed[name] = 0
+        self._doubt(name)
         self._bound(name)
         self._bounds[name], self._pushed[name] = 0, None
         self._views.pop(name, None)
@@ -191,7 +194,7 @@ class CacheBank(nn.Module):
             self._bounds[name] = self.sizes[name]
             if self._pushed[name] is None:
                 self._loaded.add(name)
-            self._pushed[name] = 0
+            self._doubt(name)
         return self._bounds[name]
 
     def _set_bound(self, name, bound):
@@ -209,20 +212,26 @@ class CacheBank(nn.Module):
                                                 _lib.raw_stream(device.index)), "mi_cache_in_order")
         return bool(order)
 
-    def _told(self, name):
-        """How many rows of the bank's end are in the order of their pushes: None for all, as far as the host knows."""
-        pushed = self._pushed[name]
-        return pushed if pushed is None and name not in self._mixed else 0 if name in self._captured else pushed
+    def _doubt(self, name):
+        self._pushed[name] = self._padded[name] = 0
 
-    def _check_order(self, name, view, counts, T, device):
+    def _told(self, name, capturing=False, given=False):
+        """How many rows of the bank's end are in the order of their pushes: None for all, as far as the host knows.  ``given``: the rows
+        asked for are counted on the device, as those of their push were."""
+        pushed = self._pushed[name]
+        if pushed is None and (capturing or name not in self._mixed):
+            return None
+        if name in self._captured and not capturing:       # a replay may have come between; a graph's own pushes come before its attention
+            return 0
+        return pushed + self._padded[name] if given else pushed
+
+    def _check_order(self, name, view, counts, T, device, given):
         """Refuses causal attention of T rows where slots do not say which rows were pushed before which.  They do until rows are evicted,
         and the rows pushed since then do; a look at the device says the same of others."""
-        told = self._told(name)
-        if told is None:
+        if self._pushed[name] is None and name not in self._mixed:
             return
         capturing = torch.cuda.is_current_stream_capturing()
-        if capturing:
-            told = self._pushed[name]                                      # a graph's own pushes come before its attention
+        told = self._told(name, capturing, given)
         if told is None or T <= told:
             return
         text = (f"CacheBank.attend: the last rows of bank {name!r} are not the rows pushed last, in their order, since an evict moved rows: causal "
@@ -252,10 +261,10 @@ class CacheBank(nn.Module):
         if key.shape != value.shape or key.dtype != value.dtype:
             raise ValueError(f"CacheBank.push: key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} differ")
         T, k = key.shape[2], self.sizes[name]
-        least = T                                       # rows that every sequence gets, for all the host knows of a tensor
+        least = T if counts is None else 0              # rows that every sequence gets, for all the host knows
         if counts is not None and not isinstance(counts, torch.Tensor):
             counts = [int(n) for n in counts]
-            least = min(counts, default=T)
+            least = min(counts, default=0)
         counts = self._counts(counts, key.shape[0], T, device)
         with _on(device):
             if not self._changes(name):
@@ -279,6 +288,7 @@ class CacheBank(nn.Module):
                                                 None if not held else out[1].data_ptr(), _lib.raw_stream(device.index)), "mi_cache_push")
             if self._pushed[name] is not None:
                 self._pushed[name] += least
+                self._padded[name] += T - least
         return out if held else None
 
     def attend(self, name, query, counts=None, scale=None, causal=True, accumulate=False):
@@ -309,6 +319,7 @@ class CacheBank(nn.Module):
         scale = dim ** -0.5 if scale is None else float(scale)
         query = query.detach()
         T, group = query.shape[2], query.shape[1] // heads
+        given = isinstance(counts, torch.Tensor)
         counts = self._counts(counts, batch, T, device)
         L = _lib.lib()
         with _on(device):
@@ -317,7 +328,7 @@ class CacheBank(nn.Module):
             if T == 0:
                 return out
             if causal and T > 1:
-                self._check_order(name, view, counts, T, device)
+                self._check_order(name, view, counts, T, device, given)
             step, out_strides = 16 // out.element_size(), _strides(out)
             if out.stride(3) != 1 or out_strides[0] % step or out_strides[1] % step or out_strides[2] % step:
                 out = torch.empty(query.shape, dtype=query.dtype, device=device)
@@ -362,7 +373,10 @@ class CacheBank(nn.Module):
             bound = self.sizes[name]
         self._set_bound(target, min(keep, bound))
         # rows moved, for all the host knows, unless there are no more than `keep`: then they are as they were
-        moved, self._pushed[target] = bound > keep, 0 if bound > keep else self._told(name)
+        moved, told, padded = bound > keep, self._told(name), self._padded[name]
+        self._doubt(target)
+        if not moved:
+            self._pushed[target], self._padded[target] = told, padded if told else 0
         if moved or name not in self._loaded:
             self._loaded.discard(target)
         else:
@@ -392,8 +406,10 @@ class CacheBank(nn.Module):
                                                 _lib.raw_stream(device.index)), "mi_cache_trim")
         bound = self._bound(name)
         self._set_bound(name, bound if each is not None else min(number, bound))
-        if self._pushed[name] is not None:             # an empty bank is in order
-            self._pushed[name] = None if each is None and number == 0 and not captured else 0
+        if self._pushed[name] is not None:
+            self._doubt(name)
+            if each is None and number == 0 and not captured:
+                self._pushed[name] = None              # an empty bank is in order
 
     def __getitem__(self, name):
         """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""

@@ -562,3 +562,85 @@ def test_the_order_after_an_eviction_goes_by_the_fewest_rows_pushed():
     _check_out(bank.attend("kv", q.cuda(), counts=[4, 1]), *ref.attend(_np(q), [4, 1]), "bf16")
     _push(bank, ref, rs, 4, np.array([4, 4]))
     _check_out(bank.attend("kv", q.cuda()), *ref.attend(_np(q)), "bf16")
+
+
+def _by_age(ref, q, n):
+    """Causal attention by positions: query row t, pushed as the (n - t)-th last of its sequence, sees the rows pushed up to then."""
+    out = np.zeros(q.shape)
+    group = q.shape[1] // ref.heads
+    for b in range(ref.batch):
+        for h in range(ref.heads):
+            for t in range(n[b]):
+                sees = ref.position[b][h] <= ref.seen[b] - n[b] + t
+                K, V = ref.key[b][h][sees], ref.value[b][h][sees]
+                for g in range(group if sees.any() else 0):
+                    s = K @ q[b, h * group + g, t] * ref.dim ** -0.5
+                    p = np.exp(s - s.max())
+                    out[b, h * group + g, t] = p @ V / p.sum()
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(8))
+def test_programs_of_calls_in_any_order(seed):
+    """Push, attend, evict and trim at random: what is held follows the lists of the reference, and causal attention either goes by the age
+    of the rows or is refused, and then only where slots would have said something else."""
+    rs = np.random.RandomState(seed)
+    B, H, group, dim, k = 3, 2, 2, [64, 128, 72, 256][seed % 4], 96
+    bank = _ica().CacheBank()
+    bank.register("kv", dim=dim, k=k, heads=H, batch=B)
+    ref = AgedBank(B, H, dim, k)
+    refused = right = 0
+    for step in range(60):
+        op = rs.choice(["push", "push", "draft", "evict", "trim", "ask"])
+        longest = max(ref.length(b) for b in range(B))
+        if op in ("push", "draft"):
+            T = int(rs.randint(1, 9))
+            if longest + T > k:
+                op = "evict"
+            else:
+                counts = None if rs.rand() < 0.5 else [int(n) for n in rs.randint(0, T + 1, B)]
+                given = counts if counts is None or rs.rand() < 0.5 else torch.tensor(counts, device="cuda")
+                kv = [_rand(rs, (B, H, T, dim), "bf16", 0.3) for _ in range(2)]
+                bank.push("kv", kv[0].cuda(), kv[1].cuda(), counts=given)
+                ref.push(_np(kv[0]), _np(kv[1]), counts)
+                if op == "draft":
+                    q = _query(rs, ref, T, group)
+                    out = _np(bank.attend("kv", q.cuda(), counts=given, accumulate=True))
+                    want, bound, weigh = ref.attend(_np(q), counts, accumulate=True)
+                    age = _by_age(ref, _np(q), [T] * B if counts is None else counts)
+                    assert np.allclose(want, age, rtol=1e-9, atol=1e-12)
+                    assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + bound * 3).all()
+                    for b in range(B):
+                        for h in range(H):
+                            got = _np(bank.weights("kv"))[b, h, :ref.length(b)]
+                            assert (np.abs(got - ref.weight[b][h]) <= weigh[b][h] + 1e-12).all()
+                            ref.weight[b][h] = got
+        if op == "evict" and longest:
+            keep = int(rs.randint(1, longest + 2))
+            recent = int(rs.randint(0, keep + 1))
+            bank.evict("kv", keep, recent=recent)
+            ref.evict(keep, recent)
+        if op == "trim":
+            cut = [max(0, ref.length(b) - int(rs.randint(0, 6))) for b in range(B)]
+            if rs.rand() < 0.2:
+                cut = [int(rs.choice([0, 20]))] * B
+            bank.trim("kv", cut[0] if len(set(cut)) == 1 else torch.tensor(cut, device="cuda"))
+            ref.trim(cut)
+        if op == "ask":
+            T = int(rs.randint(1, 6))
+            q = _query(rs, ref, T, group)
+            age, by_slot = _by_age(ref, _np(q), [T] * B), ref.attend(_np(q))
+            in_order = all(list(ref.position[b][h][-T:]) == list(range(ref.seen[b] - min(T, ref.length(b)), ref.seen[b]))
+                           for b in range(B) for h in range(H) if ref.length(b)) or T == 1
+            try:
+                out = _np(bank.attend("kv", q.cuda()))
+                assert in_order and np.allclose(by_slot[0], age, rtol=1e-9, atol=1e-12), step
+                assert (np.abs(out - age) <= 2.0 ** -8 * np.abs(age) + by_slot[1] * 3).all()
+                right += 1
+            except RuntimeError as e:
+                assert "evict" in str(e) and not in_order, step
+                refused += 1
+        _rows_equal(bank, ref)
+        assert bank._buffers["kv_seen"].tolist() == ref.seen
+    assert right > 0
