@@ -185,9 +185,9 @@ class CacheBank(nn.Module):
             return True
         return False
 
-    def _bound(self, name) -> int:
+    def _bound(self, name, length=None) -> int:
         """The bound, where it still speaks of the lengths that the bank has; otherwise they may be anything up to ``k``."""
-        length, mark = self._buffers[f"{name}_length"], self._marks.get(name)
+        length, mark = self._buffers[f"{name}_length"] if length is None else length, self._marks.get(name)
         if mark is None or mark[0] is not length or mark[1] != length._version:
             # (writes to an inference tensor are not counted: it has no mark that holds)
             self._marks[name] = (None, 0, 0) if length.is_inference() else (length, length._version, length.data_ptr())
@@ -268,7 +268,7 @@ class CacheBank(nn.Module):
         counts = self._counts(counts, key.shape[0], T, device)
         with _on(device):
             if not self._changes(name):
-                bound = k if name in self._captured else self._bound(name)
+                bound = k if name in self._captured else self._bound(name, held_by[6])
                 if bound + T > k:                       # waits for the device
                     longest = torch.empty(1, dtype=torch.int32, device=device)
                     _lib.check(_lib.lib().mi_cache_longest(view, None if counts is None else counts.data_ptr(), T, longest.data_ptr(),
@@ -362,7 +362,7 @@ class CacheBank(nn.Module):
             raise ValueError(f"CacheBank.evict: recent={recent} outside [0, keep={keep}]")
         L = _lib.lib()
         with _on(device):
-            captured, bound = self._changes(target), self._bound(name)
+            captured, bound = self._changes(target), self._bound(name, held_by[6])
             if into is not None:
                 self._bound(into)
             ws = torch.empty(int(L.mi_cache_evict_workspace_bytes(view, keep)), dtype=torch.uint8, device=device)
@@ -404,12 +404,12 @@ class CacheBank(nn.Module):
             captured = self._changes(name)
             _lib.check(_lib.lib().mi_cache_trim(view, None if each is None else each.data_ptr(), number,
                                                 _lib.raw_stream(device.index)), "mi_cache_trim")
-        bound = self._bound(name)
-        self._set_bound(name, bound if each is not None else min(number, bound))
+        if each is None:
+            self._set_bound(name, min(number, self._bound(name, held_by[6])))
         if self._pushed[name] is not None:
             self._doubt(name)
-            if each is None and number == 0 and not captured:
-                self._pushed[name] = None              # an empty bank is in order
+            if each is None and number == 0 and not captured:      # an empty bank is in order
+                self._pushed[name] = None
 
     def __getitem__(self, name):
         """(keys, values) as the bank holds them, bfloat16 [batch, heads, k, dim] each (exact); rows not in use are zeros."""
